@@ -275,7 +275,7 @@ def _words(blocks, seed, device):
     """The random words of all elements, [blocks, 64, 4], as 64-bit integers below 2^32."""
     low = 0xFFFFFFFF
     q = torch.arange(blocks * 64, dtype=torch.int64, device=device)
-    x = ((q & low) * 0x9E3779B9 & low) ^ (seed & low)
+    x = ((q & low) ^ (seed & low)) * 0x9E3779B9 & low
     x = ((x ^ (x >> 16)) + (seed >> 32) + (q >> 32) & low) * 0x6A09E667 & low
     x = (x ^ (x >> 15))[:, None]
     w = x * torch.tensor([0xBB67AE85, 0x510E527F, 0x1F83D9AB, 0x5BE0CD19], device=device) & low
