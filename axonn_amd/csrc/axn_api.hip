@@ -6,6 +6,7 @@
 #include <cstdio>
 #include <cstring>
 
+#include "axn_checks.h"
 #include "axn_internal.h"
 
 namespace axn {
@@ -25,16 +26,6 @@ int hip_fail(hipError_t e, const char* what) {
 }
 
 namespace {
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-
-#define REQUIRE(cond, code, ...)   \
-  do {                             \
-    if (!(cond)) {                 \
-      set_error(__VA_ARGS__);      \
-      return (code);               \
-    }                              \
-  } while (0)
 
 int check_gemm(const char* name, const void* a, const void* b, const void* c,
                int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
@@ -78,30 +69,6 @@ int check_f32(const char* name, const void* a, const void* b, const void* c,
           "%s: dimension exceeds 2^31-1", name);
   REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 3u) == 0, AXN_EALIGN,
           "%s: operand pointers must be 4-byte aligned", name);
-  return AXN_OK;
-}
-
-bool known_dtype(int dt) { return dt == AXN_BF16 || dt == AXN_F16 || dt == AXN_F32; }
-
-int check_list(const char* name, const void* const* h_ptrs, const char* what,
-               const int64_t* h_sizes, int64_t n, int elem_size) {
-  for (int64_t i = 0; i < n; ++i) {
-    if (h_sizes[i] == 0) continue;
-    REQUIRE(h_ptrs[i] != nullptr, AXN_EINVAL, "%s: %s[%lld] is null", name, what,
-            (long long)i);
-    REQUIRE(((uintptr_t)h_ptrs[i] % (uintptr_t)elem_size) == 0, AXN_EALIGN,
-            "%s: %s[%lld] is not aligned to its element size", name, what,
-            (long long)i);
-  }
-  return AXN_OK;
-}
-
-int check_sizes(const char* name, const int64_t* h_sizes, int64_t n) {
-  REQUIRE(n >= 0, AXN_EINVAL, "%s: negative tensor count", name);
-  REQUIRE(n == 0 || h_sizes != nullptr, AXN_EINVAL, "%s: null size array", name);
-  for (int64_t i = 0; i < n; ++i)
-    REQUIRE(h_sizes[i] >= 0, AXN_EINVAL, "%s: sizes[%lld] is negative", name,
-            (long long)i);
   return AXN_OK;
 }
 
