@@ -112,6 +112,30 @@ SYMBOLS = {
     "axn_mt_scale": (_int, [_pp, _pi64, _i64, _int, _f32, _vp, _int, _vp]),
 }
 
+# The same for include/axn_ext.h, which has a version of its own.
+EXT_ABI_VERSION = 1
+ADAMW8_BLOCK = 256
+
+
+class AdamWHParams(ctypes.Structure):
+    """Mirror of axn_adamw_hparams."""
+
+    _fields_ = [(name, _f32) for name in ("lr_over_bc1", "inv_sqrt_bc2", "one_minus_beta1", "beta2", "one_minus_beta2",
+                                          "eps", "keep")]
+
+
+EXT_SYMBOLS = {
+    "axn_ext_abi_version": (_int, []),
+    "axn_layer_norm_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _i64, _i64, _i64, _i64, _f32, _vp]),
+    "axn_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "axn_layer_norm_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _i64, _i64, _i64, _i64, _i64,
+                                  _vp, _sz, _vp]),
+    "axn_mt_adamw": (_int, [_pp, _pp, _pp, _pp, _pp, _pi64, _i64, _int, _int, _f32, _vp, _c.POINTER(AdamWHParams), _vp]),
+    "axn_mt_adamw8": (_int, [_pp, _pp, _pp, _pp, _pp, _pi64, _i64, _int, _int, _f32, _c.c_uint64, _vp,
+                             _c.POINTER(AdamWHParams), _vp]),
+    "axn_adamw8_moments": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _vp]),
+}
+
 _lib = None
 _probe_lib = None
 # axn_fast.so (csrc/fast.cpp): the host side of the usual Linear calls, same kernels.  None before `load` and where it is
@@ -190,7 +214,9 @@ def load():
                 "libaxn_gfx950.so has ABI version %d, this package needs %d"
                 % (lib.axn_abi_version(), ABI_VERSION)
             )
-        for name, (restype, argtypes) in SYMBOLS.items():
+        if not hasattr(lib, "axn_ext_abi_version") or lib.axn_ext_abi_version() != EXT_ABI_VERSION:
+            raise ImportError("libaxn_gfx950.so does not have version %d of the entry points of axn_ext.h" % EXT_ABI_VERSION)
+        for name, (restype, argtypes) in {**SYMBOLS, **EXT_SYMBOLS}.items():
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes

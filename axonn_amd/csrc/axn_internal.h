@@ -7,6 +7,7 @@
 #include <atomic>
 
 #include "axn.h"
+#include "axn_ext.h"
 
 namespace axn {
 
@@ -307,6 +308,25 @@ int launch_mt_scale(void* const* h_g, const int64_t* h_sizes, int64_t n,
                     int g_dtype, float inv_scale, const axn_scan_result* scan,
                     int use_clip, hipStream_t stream);
 
+// ---- AdamW (adamw.hip) ------------------------------------------------------
+int launch_mt_adamw(const void* const* h_g, void* const* h_p, void* const* h_m, void* const* h_v, void* const* h_plow,
+                    const int64_t* h_sizes, int64_t n, int g_dtype, int plow_dtype, float inv_scale,
+                    const axn_scan_result* scan, const axn_adamw_hparams& hp, hipStream_t stream);
+int launch_mt_adamw8(const void* const* h_g, void* const* h_p, void* const* h_codes, void* const* h_exponents,
+                     void* const* h_plow, const int64_t* h_sizes, int64_t n, int g_dtype, int plow_dtype, float inv_scale,
+                     uint64_t seed, const axn_scan_result* scan, const axn_adamw_hparams& hp, hipStream_t stream);
+int launch_adamw8_moments(const void* codes, const void* exponents, void* m, void* v, int dtype, int64_t n,
+                          hipStream_t stream);
+
+// ---- layer norm (layer_norm.hip) ----------------------------------------------
+// wide: parameters and their gradients are fp32 (else of dtype).
+int launch_layer_norm_fwd(const void* x, const void* r, const void* w, const void* b, void* y, void* h, float* mean,
+                          float* rstd, int dtype, bool wide, int64_t M, int64_t N, int64_t ldx, int64_t ldr, float eps,
+                          hipStream_t stream);
+size_t layer_norm_bwd_workspace_bytes(int64_t M, int64_t N);
+int launch_layer_norm_bwd(const void* dy, const void* h, const void* w, const float* mean, const float* rstd,
+                          const void* dsum, void* dx, void* dw, void* db, int dtype, bool wide, int64_t M, int64_t N,
+                          int64_t lddy, int64_t ldh, int64_t ldsum, void* ws, hipStream_t stream);
 
 // The dynamic LDS size a kernel may ask for is an attribute of the kernel on a device: set
 // on a kernel's first launch on each device, not on every launch.  `done` is the

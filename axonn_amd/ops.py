@@ -6,6 +6,7 @@ returns.  None of the arithmetic happens here, and nothing here falls back to a
 torch op: tensors that are not on a GPU are rejected.
 """
 
+import contextlib
 import functools
 
 import torch
@@ -753,6 +754,119 @@ def embedding_renorm_(weight, ids, max_norm, norm_type=2.0):
     return weight
 
 
+# ------------------------------------------------------------ layer norm -----
+_NOTHING = contextlib.nullcontext()
+
+
+def _device_of(name, first, *others):
+    """The tensors' one device, as the context to launch in: the library runs on the current device's stream."""
+    device = first.device
+    if device.type != "cuda":
+        _require_gpu(first)
+    for t in others:
+        if t is not None and t.device != device:
+            _require_gpu(t)
+            raise ValueError("%s: operands on %s and %s" % (name, device, t.device))
+    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _norm_params(name, dtype, N, weight, bias):
+    """Type code of a norm's parameters, of the rows' type or fp32."""
+    param = None
+    for what, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.dtype != dtype and p.dtype != torch.float32:
+            raise TypeError("%s: %s is %s, expected %s or fp32" % (name, what, p.dtype, dtype))
+        if p.dim() != 1 or p.shape[0] != N:
+            raise ValueError("%s: %s is %s, expected %d elements" % (name, what, tuple(p.shape), N))
+        if param is not None and p.dtype != param:
+            raise TypeError("%s: weight is %s but bias is %s" % (name, param, p.dtype))
+        param = p.dtype
+    return param or dtype
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, residual=None, save=True):
+    """(h - mean) rstd weight + bias over the last dimension of h = x, or of h = x + residual rounded to their type.
+    x [M, N] of bf16, fp16 or fp32, weight and bias [N] of that type or fp32.  Returns (y, h, mean, rstd): h is None
+    without a residual, mean and rstd (fp32 [M], what `layer_norm_bwd` needs) are None unless `save`."""
+    name = "layer_norm_fwd"
+    where = _device_of(name, x, weight, bias, residual)
+    code = nv.dtype_code(x.dtype)
+    x, ldx = _rows(x)
+    M, N = x.shape
+    if N == 0:
+        raise ValueError("%s: rows without elements" % name)
+    param = _norm_params(name, x.dtype, N, weight, bias)
+    weight, bias = _dense(weight), _dense(bias)
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    h, ldr, mean, rstd = None, 0, None, None
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise ValueError("%s: residual is %s %s, expected %s %s" % (name, residual.dtype, tuple(residual.shape), x.dtype,
+                                                                       tuple(x.shape)))
+        residual, ldr = _rows(residual)
+        h = torch.empty_like(y)
+    if save:
+        mean, rstd = torch.empty((2, M), dtype=torch.float32, device=x.device)
+    with where:
+        nv.call("axn_layer_norm_fwd", nv.ptr(x), nv.ptr(residual), nv.ptr(weight), nv.ptr(bias), nv.ptr(y), nv.ptr(h),
+                nv.ptr(mean), nv.ptr(rstd), code, nv.dtype_code(param), M, N, ldx, ldr, eps, nv.current_stream())
+    return y, h, mean, rstd
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_workspace_bytes(M, N):
+    return nv.load().axn_layer_norm_bwd_workspace_bytes(M, N)
+
+
+def layer_norm_bwd(dy, h, weight, mean, rstd, dsum=None, want_dx=True, want_dweight=True, want_dbias=True,
+                   param_dtype=None):
+    """Gradients of `layer_norm_fwd` for dy [M, N], h its normalised rows (x, or the sum) and their statistics: (dx,
+    dweight, dbias), None for what is not wanted.  dsum is the gradient that reaches the sum from elsewhere; dx is then
+    that of x and of the residual.  dweight and dbias are of weight's type (`param_dtype` without one: the rows')."""
+    name = "layer_norm_bwd"
+    where = _device_of(name, dy, h, weight, mean, rstd, dsum)
+    code = nv.dtype_code(dy.dtype)
+    M, N = dy.shape
+    for what, t in (("h", h), ("dsum", dsum)):
+        if t is not None and (t.dtype != dy.dtype or t.shape != dy.shape):
+            raise ValueError("%s: %s is %s %s, dy %s %s" % (name, what, t.dtype, tuple(t.shape), dy.dtype, tuple(dy.shape)))
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.shape != (M,):
+            raise ValueError("%s: mean and rstd must be fp32 with %d elements" % (name, M))
+    param = _norm_params(name, dy.dtype, N, weight, None) if weight is not None else param_dtype or dy.dtype
+    if param not in (dy.dtype, torch.float32):
+        raise TypeError("%s: gradients of parameters must be %s or fp32, got %s" % (name, dy.dtype, param))
+    if N == 0:
+        raise ValueError("%s: rows without elements" % name)
+    if not (want_dx or want_dweight or want_dbias):
+        return None, None, None
+    dy, lddy = _rows(dy)
+    h, ldh = _rows(h)
+    weight, mean, rstd, ldsum = _dense(weight), _dense(mean), _dense(rstd), 0
+    if dsum is not None:
+        dsum, ldsum = _rows(dsum)
+    dx = torch.empty((M, N), dtype=dy.dtype, device=dy.device) if want_dx else None
+    dweight = torch.empty(N, dtype=param, device=dy.device) if want_dweight else None
+    dbias = torch.empty(N, dtype=param, device=dy.device) if want_dbias else None
+    ws, ws_bytes = None, 0
+    if want_dweight or want_dbias:
+        ws_bytes = _norm_workspace_bytes(M, N)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if ws_bytes else None
+    if M == 0 and not (want_dweight or want_dbias):
+        return dx, None, None
+    with where:
+        nv.call("axn_layer_norm_bwd", nv.ptr(dy), nv.ptr(h), nv.ptr(weight), nv.ptr(mean), nv.ptr(rstd), nv.ptr(dsum),
+                nv.ptr(dx), nv.ptr(dweight), nv.ptr(dbias), code, nv.dtype_code(param), M, N, lddy, ldh, ldsum, nv.ptr(ws),
+                ws_bytes, nv.current_stream())
+    return dx, dweight, dbias
+
+
 # ---------------------------------------------------------- multi-tensor -----
 class ScanResult:
     """Device-resident axn_scan_result (32 bytes) with typed views."""
@@ -883,3 +997,114 @@ def adam_hparams(step, lr, beta1, beta2, eps, weight_decay):
         eps=eps,
         weight_decay=weight_decay,
     )
+
+
+# ----------------------------------------------------------------- AdamW -----
+def _step_lists(name, grads, params32, params_lowp, *state):
+    """Checks of the lists of a step that both kinds of moments share; (gradient, copy) type codes."""
+    n = len(grads)
+    lists = (grads, params32) + state + (() if params_lowp is None else (params_lowp,))
+    if any(len(t) != n for t in lists):
+        raise ValueError("%s: list lengths differ" % name)
+    device = grads[0].device
+    for tensors in lists:
+        dtype = tensors[0].dtype
+        for t in tensors:
+            if t.dtype != dtype:
+                raise TypeError("%s: a list holds %s and %s" % (name, dtype, t.dtype))
+            if t.device != device or not t.is_contiguous():
+                _require_gpu(t)
+                raise ValueError("%s: contiguous tensors on one device expected" % name)
+    _require_gpu(grads[0])
+    if params32[0].dtype != torch.float32:
+        raise TypeError("%s: weights must be fp32, got %s" % (name, params32[0].dtype))
+    for same in (params32,) + (() if params_lowp is None else (params_lowp,)):
+        if any(g.numel() != t.numel() for g, t in zip(grads, same)):
+            raise ValueError("%s: gradient and parameter sizes differ" % name)
+    return nv.dtype_code(grads[0].dtype), nv.BF16 if params_lowp is None else nv.dtype_code(params_lowp[0].dtype)
+
+
+def adamw_hparams(step, lr, beta1, beta2, eps, weight_decay):
+    """Host-side scalars of AdamW step number `step` (1-based), in Python doubles as `adam_hparams`."""
+    return nv.AdamWHParams(
+        lr_over_bc1=lr / (1.0 - beta1 ** step),
+        inv_sqrt_bc2=1.0 / (1.0 - beta2 ** step) ** 0.5,
+        one_minus_beta1=1.0 - beta1,
+        beta2=beta2,
+        one_minus_beta2=1.0 - beta2,
+        eps=eps,
+        keep=1.0 - lr * weight_decay,
+    )
+
+
+def mt_adamw(grads, params32, exp_avg, exp_avg_sq, params_lowp, hparams, inv_scale=1.0, scan=None):
+    """One fused AdamW pass over the lists (axn_mt_adamw in include/axn_ext.h): gradients of one type, fp32 weights and
+    moments, `params_lowp` a bf16 or fp16 copy of the weights or None; hparams from `adamw_hparams`; scan from `mt_scan`
+    clips, and skips the whole step on the device after an overflow."""
+    name = "mt_adamw"
+    if len(grads) == 0:
+        return
+    gdt, pdt = _step_lists(name, grads, params32, params_lowp, exp_avg, exp_avg_sq)
+    for what, moments in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)):
+        if moments[0].dtype != torch.float32:
+            raise TypeError("%s: %s must be fp32, got %s" % (name, what, moments[0].dtype))
+        if any(m.numel() != p.numel() for m, p in zip(moments, params32)):
+            raise ValueError("%s: moment and parameter sizes differ" % name)
+    with _device_of(name, grads[0], scan.buf if scan is not None else None):
+        nv.call("axn_mt_adamw", nv.ptr_array(grads), nv.ptr_array(params32), nv.ptr_array(exp_avg),
+                nv.ptr_array(exp_avg_sq), None if params_lowp is None else nv.ptr_array(params_lowp), nv.size_array(grads),
+                len(grads), gdt, pdt, float(inv_scale), scan.ptr() if scan is not None else None, hparams,
+                nv.current_stream())
+
+
+def adamw8_state(numel, device=None):
+    """Zero 8-bit moments of a tensor of `numel` elements: (codes [blocks, 512], exponents [blocks, 2]), blocks of 256
+    elements.  Views of whole blocks (`codes[a:b]`, `exponents[a:b]`) are moments too."""
+    blocks = -(-numel // nv.ADAMW8_BLOCK)
+    device = "cuda" if device is None else device
+    return (torch.zeros((blocks, 2 * nv.ADAMW8_BLOCK), dtype=torch.uint8, device=device),
+            torch.zeros((blocks, 2), dtype=torch.uint8, device=device))
+
+
+def _adamw8_blocks(name, codes, exponents, numel):
+    blocks = -(-numel // nv.ADAMW8_BLOCK)
+    for what, t, per in (("codes", codes, 2 * nv.ADAMW8_BLOCK), ("exponents", exponents, 2)):
+        if t.dtype != torch.uint8 or t.numel() != blocks * per:
+            raise ValueError("%s: %s must hold %d bytes for %d elements, got %d of %s"
+                             % (name, what, blocks * per, numel, t.numel(), t.dtype))
+
+
+def mt_adamw8(grads, params32, codes, exponents, params_lowp, hparams, seed, inv_scale=1.0, scan=None):
+    """`mt_adamw` with moments in 8 bits (axn_mt_adamw8 in include/axn_ext.h), a list of each tensor's codes and one of
+    its exponents, from `adamw8_state`.  `seed` (64 bits) makes the random words of the rounding: another one for every
+    step; equal calls give equal bits."""
+    name = "mt_adamw8"
+    if len(grads) == 0:
+        return
+    gdt, pdt = _step_lists(name, grads, params32, params_lowp, codes, exponents)
+    for g, c, e in zip(grads, codes, exponents):
+        _adamw8_blocks(name, c, e, g.numel())
+    with _device_of(name, grads[0], scan.buf if scan is not None else None):
+        nv.call("axn_mt_adamw8", nv.ptr_array(grads), nv.ptr_array(params32), nv.ptr_array(codes),
+                nv.ptr_array(exponents), None if params_lowp is None else nv.ptr_array(params_lowp), nv.size_array(grads),
+                len(grads), gdt, pdt, float(inv_scale), seed, scan.ptr() if scan is not None else None, hparams,
+                nv.current_stream())
+
+
+def adamw8_moments(codes, exponents, numel=None, dtype=torch.float32):
+    """The moments that 8-bit codes stand for, (exp_avg, exp_avg_sq), flat, of the first `numel` elements (all of them
+    without one).  fp32, or bf16, whose mantissa holds a code's."""
+    name = "adamw8_moments"
+    where = _device_of(name, codes, exponents)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("%s: moments come as fp32 or bf16, not %s" % (name, dtype))
+    if not (codes.is_contiguous() and exponents.is_contiguous()):
+        raise ValueError("%s: contiguous codes and exponents expected" % name)
+    if numel is None:
+        numel = codes.numel() // 2
+    _adamw8_blocks(name, codes, exponents, numel)
+    m, v = (torch.empty(numel, dtype=dtype, device=codes.device) for _ in range(2))
+    with where:
+        nv.call("axn_adamw8_moments", nv.ptr(codes), nv.ptr(exponents), nv.ptr(m), nv.ptr(v), nv.dtype_code(dtype), numel,
+                nv.current_stream())
+    return m, v

@@ -1,4 +1,5 @@
-"""Mixed-precision Adam with the reference's `CPUAdam` interface (axonn/optim.py).
+"""Mixed-precision Adam with the reference's `CPUAdam` interface (axonn/optim.py), and AdamW
+with moments in 32 or in 8 bits over the same buffers.
 
 The reference keeps fp32 master weights and Adam moments in pinned host memory
 and streams them through four GPU staging buffers in 16 M-element buckets,
@@ -22,6 +23,7 @@ buckets) and an overflow skips the whole step, not single buckets.
 import torch
 from torch.optim.optimizer import Optimizer
 
+from . import _native as nv
 from . import ops
 from .inter_layer import LossScaler, sync_scale
 from .utils import _coalesce_and_reassign
@@ -94,13 +96,18 @@ class CPUAdam(Optimizer):
             group.setdefault("amsgrad", False)
 
     # -- layout -------------------------------------------------------------
+    _span = None   # elements that a parameter of so many takes in the flat buffers (None: as many)
+
+    def _room(self, n):
+        return n if self._span is None else self._span(n)
+
     def calculate_group_offsets(self):
         """Cumulative element counts of the param groups (optim.py:59-65)."""
         self.group_offsets = [0] * (len(self.param_groups) + 1)
         for i in range(1, len(self.group_offsets)):
             group_num_params = 0
             for param in self.param_groups[i - 1]["params"]:
-                group_num_params += param.nelement()
+                group_num_params += self._room(param.nelement())
             self.group_offsets[i] = self.group_offsets[i - 1] + group_num_params
 
     def _build_flat_buffers(self):
@@ -118,7 +125,7 @@ class CPUAdam(Optimizer):
             raise RuntimeError("CPUAdam's kernels run on the GPU; move the model to the GPU first")
         with torch.no_grad():
             # flat low-precision weights; every p.data becomes a view into it
-            self.model_params_fp16 = _coalesce_and_reassign(all_params)
+            self.model_params_fp16 = _coalesce_and_reassign(all_params, self._span)
             total = self.model_params_fp16.numel()
             if self._lowp_dtype == torch.float32:
                 # fp32 model: the model weights are the master weights
@@ -126,8 +133,7 @@ class CPUAdam(Optimizer):
             else:
                 self.model_params_fp32 = self.model_params_fp16.float()
             self.model_grads_fp16 = torch.zeros(total, dtype=self._lowp_dtype, device=device)
-            self.exp_avg = torch.zeros(total, dtype=torch.float32, device=device)
-            self.exp_avg_sq = torch.zeros(total, dtype=torch.float32, device=device)
+            self._make_moments(total, device)
             offset = 0
             self._views = []
             self._params = all_params
@@ -141,8 +147,12 @@ class CPUAdam(Optimizer):
                 self._views.append((offset, n))
                 if n:
                     self._grad_views.append(flat_view)
-                offset += n
+                offset += self._room(n)
         self._writes_lowp = self._lowp_dtype != torch.float32
+
+    def _make_moments(self, total, device):
+        self.exp_avg = torch.zeros(total, dtype=torch.float32, device=device)
+        self.exp_avg_sq = torch.zeros(total, dtype=torch.float32, device=device)
 
     def empty_param_state(self, param):
         """Zeroed Adam state for a slice (optim.py:67-78); states live in HBM."""
@@ -165,6 +175,19 @@ class CPUAdam(Optimizer):
     def _group_slices(self, group_no):
         lo, hi = self.group_offsets[group_no], self.group_offsets[group_no + 1]
         return lo, hi
+
+    def _parts(self, lo, hi, *flats):
+        """One-element lists of the flat buffers' elements lo to hi."""
+        whole = hi - lo == self.model_grads_fp16.numel()   # one group: the buffers themselves
+        return [[t if whole else t[lo:hi]] for t in flats]
+
+    def _update(self, group_no, t, lo, hi, inv_scale, scan):
+        """Step number t of one param group, elements lo to hi of the flat buffers."""
+        group = self.param_groups[group_no]
+        hp = ops.adam_hparams(t, group["lr"], *group["betas"], group["eps"], group["weight_decay"])
+        g, p, m, v, low = self._parts(lo, hi, self.model_grads_fp16, self.model_params_fp32, self.exp_avg,
+                                      self.exp_avg_sq, self.model_params_fp16)
+        ops.mt_adam(g, p, m, v, low if self._writes_lowp else None, hp, inv_scale=inv_scale, scan=scan)
 
     def _relink_gradients(self):
         """The step reads the flat gradient buffer; a parameter's `.grad` is a view into
@@ -199,7 +222,6 @@ class CPUAdam(Optimizer):
         assert closure is None, "AxoNN CPUAdam does not support closure yet"
         self._relink_gradients()
         inv_scale = 1.0 / self.scaler.loss_scale
-        grads = self.model_grads_fp16
         max_norm = float(self.max_grad_norm) if self.max_grad_norm else 0.0
         need_scan = self.dynamic_loss_scale or max_norm > 0.0
         scan = None
@@ -216,13 +238,7 @@ class CPUAdam(Optimizer):
             lo, hi = self._group_slices(group_no)
             if hi == lo:
                 continue
-            beta1, beta2 = group["betas"]
-            hp = ops.adam_hparams(t, group["lr"], beta1, beta2, group["eps"],
-                                  group["weight_decay"])
-            whole = hi - lo == grads.numel()   # one group: the buffers themselves
-            g, p, m, v, low = ([t if whole else t[lo:hi]] for t in (
-                grads, self.model_params_fp32, self.exp_avg, self.exp_avg_sq, self.model_params_fp16))
-            ops.mt_adam(g, p, m, v, low if self._writes_lowp else None, hp, inv_scale=inv_scale, scan=scan)
+            self._update(group_no, t, lo, hi, inv_scale, scan)
         skipped = False
         if scan is not None:
             skipped = bool(scan.found_inf.item())  # one 4-byte read back per step
@@ -237,3 +253,67 @@ class CPUAdam(Optimizer):
         """Global 2-norm of the unscaled gradients seen by the last step (a
         0-dim device tensor), when the step scanned them."""
         return None if self._scan is None else self._scan.total_norm.clone()
+
+
+class AdamW(CPUAdam):
+    """Adam whose weight decay acts on the weights themselves, p <- (1 - lr weight_decay) p before
+    the step, over the same flat buffers, with the same loss scaling, clipping and skipped steps.
+
+    `state_bits`: 32 keeps the moments in fp32 (`exp_avg`, `exp_avg_sq`), 8 keeps them as codes of
+    8 bits with an exponent byte for each 256 elements and moment (`codes`, `exponents`; 2 bytes an
+    element instead of 8).  Codes are rounded stochastically, `seed` and the step's number make the
+    random words: runs with equal seeds are equal bit by bit.  Every parameter then starts at a
+    whole block, so `model_params_fp32` and its like have zeros between the parameters."""
+
+    def __init__(
+        self,
+        params,
+        lr=1e-3,
+        betas=(0.9, 0.999),
+        eps=1e-8,
+        weight_decay=1e-2,
+        max_grad_norm=None,
+        loss_scaler=None,
+        dynamic_loss_scale=None,
+        state_bits=32,
+        seed=0,
+    ):
+        if state_bits not in (8, 32):
+            raise ValueError("Invalid number of bits of the moments: {}".format(state_bits))
+        if state_bits == 8 and not eps > 0.0:
+            raise ValueError("8-bit moments need a positive epsilon, got {}".format(eps))
+        self.state_bits, self.seed = state_bits, int(seed)
+        if state_bits == 8:
+            self._span = lambda n: -(-n // nv.ADAMW8_BLOCK) * nv.ADAMW8_BLOCK
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm,
+                         loss_scaler=loss_scaler, dynamic_loss_scale=dynamic_loss_scale)
+
+    def _make_moments(self, total, device):
+        if self.state_bits == 8:
+            self.codes, self.exponents = ops.adamw8_state(total, device)
+        else:
+            super()._make_moments(total, device)
+
+    def _step_seed(self, t, group_no):
+        odd = 0x9E3779B97F4A7C15
+        return ((self.seed * odd + t) * odd + group_no) * odd % (1 << 64)
+
+    def _update(self, group_no, t, lo, hi, inv_scale, scan):
+        group = self.param_groups[group_no]
+        hp = ops.adamw_hparams(t, group["lr"], *group["betas"], group["eps"], group["weight_decay"])
+        g, p, low = self._parts(lo, hi, self.model_grads_fp16, self.model_params_fp32, self.model_params_fp16)
+        low = low if self._writes_lowp else None
+        if self.state_bits == 8:
+            first, last = lo // nv.ADAMW8_BLOCK, hi // nv.ADAMW8_BLOCK
+            ops.mt_adamw8(g, p, [self.codes[first:last]], [self.exponents[first:last]], low, hp,
+                          self._step_seed(t, group_no), inv_scale=inv_scale, scan=scan)
+        else:
+            m, v = self._parts(lo, hi, self.exp_avg, self.exp_avg_sq)
+            ops.mt_adamw(g, p, m, v, low, hp, inv_scale=inv_scale, scan=scan)
+
+    def moments(self):
+        """(exp_avg, exp_avg_sq) of every parameter, in fp32 and its shape: with 32 bits views of the
+        flat buffers, with 8 bits what the codes stand for now."""
+        m, v = (self.exp_avg, self.exp_avg_sq) if self.state_bits == 32 else ops.adamw8_moments(self.codes, self.exponents)
+        return [(m[offset:offset + n].view(p.shape), v[offset:offset + n].view(p.shape))
+                for p, (offset, n) in zip(self._params, self._views)]
