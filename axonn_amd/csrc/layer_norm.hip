@@ -153,9 +153,190 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_dparam_sum_kernel(const Norm
   }
 }
 
+// ---------------------------------------------------------- vector kernels --
+// A row lies in the registers of TPR threads, K vectors of 16 bytes in each, and is read once.
+// Vector v of a row holds its elements from v VEC on, but the last one ends with the row and
+// overlaps the one before: `twice` of its elements are in both, count once in sums and are
+// stored by both with one value.  Rows may start anywhere: the accesses are declared to be
+// aligned to an element only, which gfx950 reads in one instruction all the same.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  typedef T Type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::Type load_vec(const T* p) {
+  return *(const typename Vec<T>::Type*)p;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, typename Vec<T>::Type v) {
+  *(typename Vec<T>::Type*)p = v;
+}
+// VEC parameters from element i on, as floats.
+template <typename T>
+__device__ __forceinline__ void load_params(const void* p, int wide, int64_t i, float (&out)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  if (sizeof(T) == 4 || wide) {
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      const auto v = load_vec((const float*)p + i + 4 * j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[4 * j + e] = v[e];
+    }
+  } else {
+    const auto v = load_vec((const T*)p + i);
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = (float)v[e];
+  }
+}
+
+// Where vector v of rows of n elements starts, and how many of its elements others have.  A
+// vector behind the row is its last one again, none of its elements its own, so that loads need
+// no branch around them, which would have each wait for the one before.
+struct Span {
+  int first, twice;
+};
+template <int VEC>
+__device__ __forceinline__ Span span_of(int v, int n) {
+  const int first = min(v * VEC, n - VEC);
+  return {first, min(v * VEC - first, VEC)};
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// The sum over 16 neighbouring lanes, or over the wave, in all of them: rotations by 8, 4, 2
+// and 1 within the rows of 16 lanes, which no LDS access or wait is behind.
+__device__ __forceinline__ float row16_sum(float x) {
+  x = dpp_add<0x128>(x);
+  x = dpp_add<0x124>(x);
+  x = dpp_add<0x122>(x);
+  return dpp_add<0x121>(x);
+}
+__device__ __forceinline__ float lane_of(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+__device__ __forceinline__ float wave64_sum(float x) {
+  x = row16_sum(x);
+  return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
+}
+// The sum over the TPR threads that hold a row; rows of several waves meet in `shared`, which
+// has a place for every wave and is not written again before the next barrier but one.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float x, float* shared) {
+  if (TPR == 16) return row16_sum(x);
+  x = wave64_sum(x);
+  if (TPR == 64) return x;
+  constexpr int WAVES = TPR / 64;
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) shared[wave] = x;
+  __syncthreads();
+  const int first = wave / WAVES * WAVES;
+  x = 0.0f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) x += shared[first + w];
+  return x;
+}
+
+template <typename T, int TPR, int K, bool RES>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_rows_kernel(const NormArgs a) {
+  constexpr int VEC = Vec<T>::N, BLOCK = TPR > 256 ? TPR : 256;
+  __shared__ float shared[2][BLOCK / 64];
+  const int t = threadIdx.x % TPR, n = (int)a.N;
+  int64_t row = block_number() * (BLOCK / TPR) + threadIdx.x / TPR;
+  const bool live = row < a.M;   // (the threads behind the last row reach the barriers, with that row)
+  if (!live) row = a.M - 1;
+  typename Vec<T>::Type x[K], r[RES ? K : 1];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const Span at = span_of<VEC>(k * TPR + t, n);
+    x[k] = load_vec((const T*)a.x + row * a.ldx + at.first);
+    if (RES) r[k] = load_vec((const T*)a.r + row * a.ldr + at.first);
+  }
+  float h[K][VEC];
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const Span at = span_of<VEC>(k * TPR + t, n);
+    if (RES) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[k][e] = (T)((float)x[k][e] + (float)r[k][e]);
+      if (live && at.twice < VEC) store_vec((T*)a.h + row * a.N + at.first, x[k]);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      h[k][e] = (float)x[k][e];
+      s += e < at.twice ? 0.0f : h[k][e];
+    }
+  }
+  const float mean = row_sum<TPR>(s, shared[0]) / (float)n;
+  s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const Span at = span_of<VEC>(k * TPR + t, n);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      h[k][e] -= mean;
+      s += e < at.twice ? 0.0f : h[k][e] * h[k][e];
+    }
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<TPR>(s, shared[1]) / (float)n + a.eps);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const Span at = span_of<VEC>(k * TPR + t, n);
+    if (!live || at.twice == VEC) continue;
+    float w[VEC], b[VEC];
+    if (a.w) load_params<T>(a.w, a.wide, at.first, w);
+    if (a.b) load_params<T>(a.b, a.wide, at.first, b);
+    typename Vec<T>::Type y;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float f = h[k][e] * rstd;
+      if (a.w) f *= w[e];
+      if (a.b) f += b[e];
+      y[e] = (T)f;
+    }
+    store_vec((T*)a.y + row * a.N + at.first, y);
+  }
+  if (live && t == 0 && a.mean) {
+    a.mean[row] = mean;
+    a.rstd[row] = rstd;
+  }
+}
+
+template <typename T, int TPR, int K>
+int norm_rows_launch(const NormArgs& a, hipStream_t stream) {
+  constexpr int BLOCK = TPR > 256 ? TPR : 256;
+  const dim3 grid = grid_of(ceil_div(a.M, BLOCK / TPR));
+  if (a.r)
+    hipLaunchKernelGGL((norm_rows_kernel<T, TPR, K, true>), grid, dim3(BLOCK), 0, stream, a);
+  else
+    hipLaunchKernelGGL((norm_rows_kernel<T, TPR, K, false>), grid, dim3(BLOCK), 0, stream, a);
+  AXN_HIP_TRY(hipGetLastError());
+  return AXN_OK;
+}
+
+// Rows of one workgroup's threads, K vectors in each: as few as hold the row.
+template <typename T>
+int norm_rows(const NormArgs& a, hipStream_t stream) {
+  const int64_t v = ceil_div(a.N, Vec<T>::N);
+  if (v <= 16) return norm_rows_launch<T, 16, 1>(a, stream);
+  if (v <= 32) return norm_rows_launch<T, 16, 2>(a, stream);
+  if (v <= 64) return norm_rows_launch<T, 64, 1>(a, stream);
+  if (v <= 128) return norm_rows_launch<T, 64, 2>(a, stream);
+  if (v <= 256) return norm_rows_launch<T, 256, 1>(a, stream);
+  if (v <= 512) return norm_rows_launch<T, 256, 2>(a, stream);
+  if (v <= 768) return norm_rows_launch<T, 256, 3>(a, stream);
+  if (v <= 1024) return norm_rows_launch<T, 256, 4>(a, stream);
+  if (v <= 2048) return norm_rows_launch<T, 1024, 2>(a, stream);
+  return norm_rows_launch<T, 1024, 4>(a, stream);
+}
+
 template <int DT>
 int norm_launch(const NormArgs& a, hipStream_t stream) {
   typedef typename Elem<DT>::type T;
+  if (a.N >= Vec<T>::N && a.N <= 4096 * Vec<T>::N) return norm_rows<T>(a, stream);
   hipLaunchKernelGGL(norm_any_kernel<T>, grid_of(a.M), dim3(ROW_THREADS), 0, stream, a);
   AXN_HIP_TRY(hipGetLastError());
   return AXN_OK;
