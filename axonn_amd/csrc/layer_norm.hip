@@ -30,6 +30,7 @@ __device__ __forceinline__ float param_at(const void* p, int wide, int64_t i) {
 }
 
 constexpr int ROW_THREADS = 256;
+constexpr int MOST_PARTS = 256;   // parts of the rows whose column sums meet in a second launch
 
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float x, float* shared) {
@@ -232,11 +233,12 @@ __device__ __forceinline__ float row_sum(float x, float* shared) {
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) shared[wave] = x;
   __syncthreads();
-  const int first = wave / WAVES * WAVES;
-  x = 0.0f;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) x += shared[first + w];
-  return x;
+  // the row's waves' sums, over and over in the lanes: rotations by less than 16 add them all
+  x = shared[wave / WAVES * WAVES + threadIdx.x % WAVES];
+  if (WAVES > 8) x = dpp_add<0x128>(x);
+  if (WAVES > 4) x = dpp_add<0x124>(x);
+  if (WAVES > 2) x = dpp_add<0x122>(x);
+  return dpp_add<0x121>(x);
 }
 
 template <typename T, int TPR, int K, bool RES>
@@ -333,6 +335,211 @@ int norm_rows(const NormArgs& a, hipStream_t stream) {
   return norm_rows_launch<T, 1024, 4>(a, stream);
 }
 
+// Backward: rows of TPR threads as above, BLOCK / TPR of them at a time in a workgroup, which goes
+// on to the rows `parts` workgroups further until there are none.  Its threads keep the sums of
+// dy xhat and dy of their columns in registers; at the end the workgroup's rows are joined in LDS
+// and its sums go to `partial`, or, from the only workgroup, to dw and db.
+// RAGGED: N is no multiple of a vector.  SUM: dsum is given.
+template <typename T, int TPR, int K, int BLOCK, bool RAGGED, bool SUM>
+__global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(const NormGradArgs a) {
+  constexpr int VEC = Vec<T>::N, ROWS = BLOCK / TPR;
+  __shared__ float meet[2][2][BLOCK / 64];
+  __shared__ float joined[ROWS > 1 ? ROWS : 1][ROWS > 1 ? TPR * VEC : 1];
+  typedef typename Vec<T>::Type V;
+  const int t = threadIdx.x % TPR, n = (int)a.N;
+  // (the row of a whole wave is a scalar: addresses are a scalar base and a lane's offset)
+  const int group = TPR >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : threadIdx.x / TPR;
+  const float inv_n = 1.0f / (float)n;
+  float w[K][VEC], dw[K][VEC], db[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const Span at = span_of<VEC>(k * TPR + t, n);
+    if (a.w) load_params<T>(a.w, a.wide, at.first, w[k]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (!a.w) w[k][e] = 1.0f;
+      dw[k][e] = db[k][e] = 0.0f;
+    }
+  }
+  struct Row {
+    V dy[K], h[K];
+    float mean, rstd;
+  };
+  auto fetch = [&](Row& r, int64_t row) {   // (behind the last row: that row again, counted as nothing)
+    row = row < a.M ? row : a.M - 1;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const Span at = span_of<VEC>(k * TPR + t, n);
+      r.dy[k] = load_vec((const T*)a.dy + row * a.lddy + at.first);
+      r.h[k] = load_vec((const T*)a.h + row * a.ldh + at.first);
+    }
+    r.mean = a.mean[row];
+    r.rstd = a.rstd[row];
+  };
+  const int64_t stride = (int64_t)a.parts * ROWS;
+  int64_t first = (int64_t)blockIdx.x * ROWS;   // the workgroup's first row of this turn
+  int turn = 0;
+  // One turn: the next one's rows are on their way while this one's are summed, if registers
+  // hold both.
+  constexpr bool AHEAD = K <= 2;
+  auto step = [&](Row& r, Row& next) -> bool {
+    const int64_t row = first + group;
+    const bool live = row < a.M, more = first + stride < a.M;
+    if (!AHEAD) fetch(r, row);
+    V extra[SUM ? K : 1];
+    if (SUM && live) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        extra[k] = load_vec((const T*)a.dsum + row * a.ldsum + span_of<VEC>(k * TPR + t, n).first);
+    }
+    if (AHEAD && more) fetch(next, row + stride);
+    float s1 = 0.0f, s2 = 0.0f;
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const Span at = span_of<VEC>(k * TPR + t, n);
+        float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float d = (float)r.dy[k][e], c = (float)r.h[k][e] - r.mean, g = d * w[k][e];
+          dw[k][e] += d * (c * r.rstd);
+          db[k][e] += d;
+          t1 += RAGGED && e < at.twice ? 0.0f : g;
+          t2 += RAGGED && e < at.twice ? 0.0f : g * c;
+        }
+        s1 += !RAGGED && at.twice ? 0.0f : t1;
+        s2 += !RAGGED && at.twice ? 0.0f : t2;
+      }
+    }
+    // dx = rstd (g - mean(g) - xhat mean(g xhat)) with xhat = c rstd
+    const float shift = row_sum<TPR>(s1, meet[turn][0]) * inv_n * r.rstd;
+    const float slope = row_sum<TPR>(s2, meet[turn][1]) * inv_n * r.rstd * r.rstd;
+    if (live && a.dx) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const Span at = span_of<VEC>(k * TPR + t, n);
+        if (at.twice == VEC) continue;
+        V out;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float c = (float)r.h[k][e] - r.mean;
+          float d = (float)r.dy[k][e] * w[k][e] * r.rstd - shift;
+          d -= c * r.rstd * slope;
+          if (SUM) d += (float)extra[k][e];
+          out[e] = (T)d;
+        }
+        store_vec((T*)a.dx + row * a.N + at.first, out);
+      }
+    }
+    first += stride;
+    turn ^= 1;
+    return more;
+  };
+  Row one, other;
+  if (AHEAD) {
+    fetch(one, first + group);
+    while (step(one, other) && step(other, one)) {
+    }
+  } else {
+    while (step(one, one)) {
+    }
+  }
+  if (!a.partial) return;
+  float* sums = a.partial + (int64_t)blockIdx.x * 2 * n;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (ROWS == 1) {   // (of elements that two vectors have, both have the same sums)
+      const Span at = span_of<VEC>(k * TPR + t, n);
+      if (at.twice == VEC) continue;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        sums[at.first + e] = dw[k][e];
+        sums[n + at.first + e] = db[k][e];
+      }
+      continue;
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) joined[group][t * VEC + e] = which == 0 ? dw[k][e] : db[k][e];
+      __syncthreads();
+      for (int c = threadIdx.x; c < TPR * VEC; c += BLOCK) {
+        const Span at = span_of<VEC>(k * TPR + c / VEC, n);
+        if (c % VEC < at.twice) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) s += joined[r][c];
+        sums[which * (int64_t)n + at.first + c % VEC] = s;
+      }
+    }
+  }
+}
+
+// The workgroups' sums added up: 32 of the 2 N columns to a workgroup, 8 threads of 4 columns,
+// 32 of them taking every 32nd part.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormGradArgs a) {
+  __shared__ float4 shared[32][8];
+  const int slice = threadIdx.x / 8, lane = threadIdx.x % 8;
+  const int64_t all = 2 * a.N, col = (block_number() * 8 + lane) * 4;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (col < all) {
+    for (int part = slice; part < a.parts; part += 32) {
+      const float* p = a.partial + (int64_t)part * all + col;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < all) s[e] += p[e];
+    }
+  }
+  shared[slice][lane] = float4{s[0], s[1], s[2], s[3]};
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  const int64_t c = block_number() * 32 + threadIdx.x;
+  if (c >= all) return;
+  float total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) total += ((const float*)&shared[i][0])[threadIdx.x];
+  void* out = c < a.N ? a.dw : a.db;
+  const int64_t i = c < a.N ? c : c - a.N;
+  if (!out) return;
+  if (a.wide) ((float*)out)[i] = total; else ((T*)out)[i] = (T)total;
+}
+
+template <typename T, int TPR, int K, int BLOCK>
+int norm_grad_rows_launch(NormGradArgs a, hipStream_t stream) {
+  const bool params = a.dw || a.db;
+  const int64_t groups = ceil_div(a.M, BLOCK / TPR);
+  a.parts = groups < MOST_PARTS ? (int)groups : MOST_PARTS;
+  if (!params) a.partial = nullptr;
+#define AXN_NORM_GRAD(RAGGED, SUM)                                                                                   \
+  hipLaunchKernelGGL((norm_grad_rows_kernel<T, TPR, K, BLOCK, RAGGED, SUM>), dim3(a.parts), dim3(BLOCK), 0, stream, a)
+  const bool ragged = a.N % Vec<T>::N != 0;
+  if (ragged && a.dsum) AXN_NORM_GRAD(true, true);
+  if (ragged && !a.dsum) AXN_NORM_GRAD(true, false);
+  if (!ragged && a.dsum) AXN_NORM_GRAD(false, true);
+  if (!ragged && !a.dsum) AXN_NORM_GRAD(false, false);
+#undef AXN_NORM_GRAD
+  AXN_HIP_TRY(hipGetLastError());
+  if (params) {
+    hipLaunchKernelGGL(norm_grad_join_kernel<T>, grid_of(ceil_div(2 * a.N, 32)), dim3(256), 0, stream, a);
+    AXN_HIP_TRY(hipGetLastError());
+  }
+  return AXN_OK;
+}
+
+template <typename T>
+int norm_grad_rows(const NormGradArgs& a, hipStream_t stream) {
+  const int64_t v = ceil_div(a.N, Vec<T>::N);
+  if (v <= 32) return norm_grad_rows_launch<T, 16, 2, 256>(a, stream);
+  if (v <= 128) return norm_grad_rows_launch<T, 64, 2, 256>(a, stream);
+  if (v <= 256) return norm_grad_rows_launch<T, 128, 2, 1024>(a, stream);
+  if (v <= 512) return norm_grad_rows_launch<T, 256, 2, 1024>(a, stream);
+  if (v <= 1024) return norm_grad_rows_launch<T, 512, 2, 1024>(a, stream);
+  if (v <= 2048) return norm_grad_rows_launch<T, 1024, 2, 1024>(a, stream);
+  return norm_grad_rows_launch<T, 1024, 4, 1024>(a, stream);
+}
+
 template <int DT>
 int norm_launch(const NormArgs& a, hipStream_t stream) {
   typedef typename Elem<DT>::type T;
@@ -345,6 +552,7 @@ int norm_launch(const NormArgs& a, hipStream_t stream) {
 template <int DT>
 int norm_grad_launch(const NormGradArgs& a, hipStream_t stream) {
   typedef typename Elem<DT>::type T;
+  if (a.M > 0 && a.N >= Vec<T>::N && a.N <= 16384) return norm_grad_rows<T>(a, stream);
   if (a.dx) {
     hipLaunchKernelGGL(norm_dx_any_kernel<T>, grid_of(a.M), dim3(ROW_THREADS), 0, stream, a);
     AXN_HIP_TRY(hipGetLastError());
@@ -363,17 +571,17 @@ int norm_grad_launch(const NormGradArgs& a, hipStream_t stream) {
   return AXN_OK;
 }
 
-// Into how many parts the rows are cut for the sums over them.
+// Into how many parts the rows are cut for the sums over them, element by element.
 int norm_grad_parts(int64_t M) {
   const int64_t parts = ceil_div(M, 16);
-  return parts > 256 ? 256 : (int)parts;
+  return parts > MOST_PARTS ? MOST_PARTS : (int)parts;
 }
 
 }  // namespace
 
 size_t layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
   if (M < 1 || N < 1) return 0;
-  return (size_t)norm_grad_parts(M) * 2 * (size_t)N * sizeof(float);
+  return (size_t)(M < MOST_PARTS ? M : MOST_PARTS) * 2 * (size_t)N * sizeof(float);
 }
 
 int launch_layer_norm_fwd(const void* x, const void* r, const void* w, const void* b, void* y, void* h, float* mean,
