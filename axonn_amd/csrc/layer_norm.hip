@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_dparam_sum_kernel(const Norm
 }
 
 // ---------------------------------------------------------- vector kernels --
-// A row lies in the registers of TPR threads, K vectors of 16 bytes in each, and is read once.
+// A row lies in the registers of 16 lanes or of several whole waves, K vectors of 16 bytes in a
+// lane, and is read once.
 // Vector v of a row holds its elements from v VEC on, but the last one ends with the row and
 // overlaps the one before: `twice` of its elements are in both, count once in sums and are
 // stored by both with one value.  Rows may start anywhere: the accesses are declared to be
@@ -203,6 +204,19 @@ __device__ __forceinline__ Span span_of(int v, int n) {
   return {first, min(v * VEC - first, VEC)};
 }
 
+// The threads of a row: SUB: 16 lanes, else `waves` whole waves (16 at most).
+template <bool SUB>
+struct RowOf {
+  int waves, lane, threads, group;   // waves of a row, this thread's place among its row's, their number, the row in the workgroup
+  __device__ __forceinline__ RowOf(int w) : waves(w) {
+    threads = SUB ? 16 : waves * 64;
+    // (the row of a whole wave is a scalar: addresses are a scalar base and a lane's offset)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    group = SUB ? (int)threadIdx.x >> 4 : wave / waves;
+    lane = SUB ? (int)threadIdx.x & 15 : (wave - group * waves) * 64 + ((int)threadIdx.x & 63);
+  }
+};
+
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float x) {
   return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
@@ -222,139 +236,190 @@ __device__ __forceinline__ float wave64_sum(float x) {
   x = row16_sum(x);
   return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
 }
-// The sum over the TPR threads that hold a row; rows of several waves meet in `shared`, which
-// has a place for every wave and is not written again before the next barrier but one.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float x, float* shared) {
-  if (TPR == 16) return row16_sum(x);
-  x = wave64_sum(x);
-  if (TPR == 64) return x;
-  constexpr int WAVES = TPR / 64;
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) shared[wave] = x;
+// COUNT sums over the threads of a row; the waves of one meet in `shared`, COUNT places for every
+// wave, which is not written again before the next barrier but one.
+template <bool SUB, int COUNT>
+__device__ __forceinline__ void row_sums(float (&x)[COUNT], const RowOf<SUB>& at, float (*shared)[16]) {
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) x[i] = SUB ? row16_sum(x[i]) : wave64_sum(x[i]);
+  if (SUB || at.waves == 1) return;
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) shared[i][threadIdx.x >> 6] = x[i];
+  }
   __syncthreads();
-  // the row's waves' sums, over and over in the lanes: rotations by less than 16 add them all
-  x = shared[wave / WAVES * WAVES + threadIdx.x % WAVES];
-  if (WAVES > 8) x = dpp_add<0x128>(x);
-  if (WAVES > 4) x = dpp_add<0x124>(x);
-  if (WAVES > 2) x = dpp_add<0x122>(x);
-  return dpp_add<0x121>(x);
-}
-
-template <typename T, int TPR, int K, bool RES>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_rows_kernel(const NormArgs a) {
-  constexpr int VEC = Vec<T>::N, BLOCK = TPR > 256 ? TPR : 256;
-  __shared__ float shared[2][BLOCK / 64];
-  const int t = threadIdx.x % TPR, n = (int)a.N;
-  int64_t row = block_number() * (BLOCK / TPR) + threadIdx.x / TPR;
-  const bool live = row < a.M;   // (the threads behind the last row reach the barriers, with that row)
-  if (!live) row = a.M - 1;
-  typename Vec<T>::Type x[K], r[RES ? K : 1];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const Span at = span_of<VEC>(k * TPR + t, n);
-    x[k] = load_vec((const T*)a.x + row * a.ldx + at.first);
-    if (RES) r[k] = load_vec((const T*)a.r + row * a.ldr + at.first);
-  }
-  float h[K][VEC];
-  float s = 0.0f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const Span at = span_of<VEC>(k * TPR + t, n);
-    if (RES) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x[k][e] = (T)((float)x[k][e] + (float)r[k][e]);
-      if (live && at.twice < VEC) store_vec((T*)a.h + row * a.N + at.first, x[k]);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      h[k][e] = (float)x[k][e];
-      s += e < at.twice ? 0.0f : h[k][e];
-    }
-  }
-  const float mean = row_sum<TPR>(s, shared[0]) / (float)n;
-  s = 0.0f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const Span at = span_of<VEC>(k * TPR + t, n);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      h[k][e] -= mean;
-      s += e < at.twice ? 0.0f : h[k][e] * h[k][e];
-    }
-  }
-  const float rstd = 1.0f / sqrtf(row_sum<TPR>(s, shared[1]) / (float)n + a.eps);
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const Span at = span_of<VEC>(k * TPR + t, n);
-    if (!live || at.twice == VEC) continue;
-    float w[VEC], b[VEC];
-    if (a.w) load_params<T>(a.w, a.wide, at.first, w);
-    if (a.b) load_params<T>(a.b, a.wide, at.first, b);
-    typename Vec<T>::Type y;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float f = h[k][e] * rstd;
-      if (a.w) f *= w[e];
-      if (a.b) f += b[e];
-      y[e] = (T)f;
-    }
-    store_vec((T*)a.y + row * a.N + at.first, y);
-  }
-  if (live && t == 0 && a.mean) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
+  for (int i = 0; i < COUNT; ++i) {
+    const float mine = shared[i][at.group * at.waves + min(lane & 15, at.waves - 1)];
+    x[i] = row16_sum((lane & 15) < at.waves ? mine : 0.0f);
   }
 }
 
-template <typename T, int TPR, int K>
-int norm_rows_launch(const NormArgs& a, hipStream_t stream) {
-  constexpr int BLOCK = TPR > 256 ? TPR : 256;
-  const dim3 grid = grid_of(ceil_div(a.M, BLOCK / TPR));
-  if (a.r)
-    hipLaunchKernelGGL((norm_rows_kernel<T, TPR, K, true>), grid, dim3(BLOCK), 0, stream, a);
-  else
-    hipLaunchKernelGGL((norm_rows_kernel<T, TPR, K, false>), grid, dim3(BLOCK), 0, stream, a);
+// RES: a residual is added.  RAGGED: N is no multiple of a vector.  A workgroup takes `rows` rows at
+// a time and goes on to those gridDim.x workgroups further; the parameters of its columns stay in
+// registers.
+template <typename T, int K, bool SUB, bool RES, bool RAGGED>
+__global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int waves, int rows) {
+  constexpr int VEC = Vec<T>::N;
+  typedef typename Vec<T>::Type V;
+  __shared__ float shared[2][2][16];
+  const RowOf<SUB> at(waves);
+  const int n = (int)a.N;
+  float w[K][VEC], b[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
+    if (a.w) load_params<T>(a.w, a.wide, first, w[k]);
+    if (a.b) load_params<T>(a.b, a.wide, first, b[k]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (!a.w) w[k][e] = 1.0f;
+      if (!a.b) b[k][e] = 0.0f;
+    }
+  }
+  struct Row {
+    V x[K], r[RES ? K : 1];
+  };
+  auto fetch = [&](Row& f, int64_t row) {   // (behind the last row: that row again)
+    row = row < a.M ? row : a.M - 1;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
+      f.x[k] = load_vec((const T*)a.x + row * a.ldx + first);
+      if (RES) f.r[k] = load_vec((const T*)a.r + row * a.ldr + first);
+    }
+  };
+  const int64_t stride = (int64_t)gridDim.x * rows;
+  int64_t begin = (int64_t)blockIdx.x * rows;   // the workgroup's first row of this turn
+  int turn = 0;
+  constexpr bool AHEAD = K <= 2;
+  auto step = [&](Row& f, Row& next) -> bool {
+    const int64_t row = begin + at.group;
+    const bool live = row < a.M, more = begin + stride < a.M;
+    if (!AHEAD) fetch(f, row);
+    if (AHEAD && more) fetch(next, row + stride);
+    float h[K][VEC], s[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const Span span = span_of<VEC>(k * at.threads + at.lane, n);
+      if (RES) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f.x[k][e] = (T)((float)f.x[k][e] + (float)f.r[k][e]);
+        if (live && span.twice < VEC) store_vec((T*)a.h + row * a.N + span.first, f.x[k]);
+      }
+      float t = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        h[k][e] = (float)f.x[k][e];
+        t += RAGGED && e < span.twice ? 0.0f : h[k][e];
+      }
+      s[0] += !RAGGED && span.twice ? 0.0f : t;
+    }
+    row_sums<SUB>(s, at, &shared[turn][0]);
+    const float mean = s[0] / (float)n;   // (of equal elements, that element)
+    s[0] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const Span span = span_of<VEC>(k * at.threads + at.lane, n);
+      float t = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        h[k][e] -= mean;
+        t += RAGGED && e < span.twice ? 0.0f : h[k][e] * h[k][e];
+      }
+      s[0] += !RAGGED && span.twice ? 0.0f : t;
+    }
+    row_sums<SUB>(s, at, &shared[turn][1]);
+    const float rstd = 1.0f / sqrtf(s[0] / (float)n + a.eps);
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const Span span = span_of<VEC>(k * at.threads + at.lane, n);
+        if (span.twice == VEC) continue;
+        V y;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) y[e] = (T)(h[k][e] * rstd * w[k][e] + b[k][e]);
+        store_vec((T*)a.y + row * a.N + span.first, y);
+      }
+      if (at.lane == 0 && a.mean) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+      }
+    }
+    begin += stride;
+    turn ^= 1;
+    return more;
+  };
+  Row one, other;
+  if (AHEAD) {
+    fetch(one, begin + at.group);
+    while (step(one, other) && step(other, one)) {
+    }
+  } else {
+    while (step(one, one)) {
+    }
+  }
+}
+
+// Waves and vectors of a lane for rows of N elements, and whether 16 lanes do.
+struct RowPlan {
+  int k, waves;
+  bool sub;
+};
+inline RowPlan plan_row(int64_t N, int vec) {
+  const int64_t v = ceil_div(N, vec);
+  if (v <= 32) return {2, 1, true};
+  if (v <= 2048) return {2, (int)ceil_div(v, 128), false};
+  return {4, (int)ceil_div(v, 256), false};
+}
+
+template <typename T, int K, bool SUB>
+int norm_rows_launch(const NormArgs& a, const RowPlan& plan, hipStream_t stream) {
+  const int rows = SUB ? 16 : plan.waves >= 4 ? 1 : 4 / plan.waves;
+  const int threads = SUB ? 256 : plan.waves * rows * 64;
+  int64_t groups = ceil_div(a.M, rows);
+  const int64_t most = 256 * (2048 / threads) / 2;
+  if (groups > most) groups = most;
+#define AXN_NORM(RES, RAGGED)                                                                              \
+  hipLaunchKernelGGL((norm_rows_kernel<T, K, SUB, RES, RAGGED>), dim3((unsigned)groups), dim3(threads), 0, \
+                     stream, a, plan.waves, rows)
+  const bool ragged = a.N % Vec<T>::N != 0;
+  if (ragged && a.r) AXN_NORM(true, true);
+  if (ragged && !a.r) AXN_NORM(false, true);
+  if (!ragged && a.r) AXN_NORM(true, false);
+  if (!ragged && !a.r) AXN_NORM(false, false);
+#undef AXN_NORM
   AXN_HIP_TRY(hipGetLastError());
   return AXN_OK;
 }
 
-// Rows of one workgroup's threads, K vectors in each: as few as hold the row.
 template <typename T>
 int norm_rows(const NormArgs& a, hipStream_t stream) {
-  const int64_t v = ceil_div(a.N, Vec<T>::N);
-  if (v <= 16) return norm_rows_launch<T, 16, 1>(a, stream);
-  if (v <= 32) return norm_rows_launch<T, 16, 2>(a, stream);
-  if (v <= 64) return norm_rows_launch<T, 64, 1>(a, stream);
-  if (v <= 128) return norm_rows_launch<T, 64, 2>(a, stream);
-  if (v <= 256) return norm_rows_launch<T, 256, 1>(a, stream);
-  if (v <= 512) return norm_rows_launch<T, 256, 2>(a, stream);
-  if (v <= 768) return norm_rows_launch<T, 256, 3>(a, stream);
-  if (v <= 1024) return norm_rows_launch<T, 256, 4>(a, stream);
-  if (v <= 2048) return norm_rows_launch<T, 1024, 2>(a, stream);
-  return norm_rows_launch<T, 1024, 4>(a, stream);
+  const RowPlan plan = plan_row(a.N, Vec<T>::N);
+  if (plan.sub) return norm_rows_launch<T, 2, true>(a, plan, stream);
+  if (plan.k == 2) return norm_rows_launch<T, 2, false>(a, plan, stream);
+  return norm_rows_launch<T, 4, false>(a, plan, stream);
 }
 
-// Backward: rows of TPR threads as above, BLOCK / TPR of them at a time in a workgroup, which goes
-// on to the rows `parts` workgroups further until there are none.  Its threads keep the sums of
-// dy xhat and dy of their columns in registers; at the end the workgroup's rows are joined in LDS
-// and its sums go to `partial`, or, from the only workgroup, to dw and db.
-// RAGGED: N is no multiple of a vector.  SUM: dsum is given.
-template <typename T, int TPR, int K, int BLOCK, bool RAGGED, bool SUM>
-__global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(const NormGradArgs a) {
-  constexpr int VEC = Vec<T>::N, ROWS = BLOCK / TPR;
-  __shared__ float meet[2][2][BLOCK / 64];
-  __shared__ float joined[ROWS > 1 ? ROWS : 1][ROWS > 1 ? TPR * VEC : 1];
+// Backward: rows as above, several at a time in a workgroup, which goes on to the rows `parts`
+// workgroups further until there are none.  Its threads keep the sums of dy xhat and dy of their
+// columns in registers; at the end the workgroup's rows are joined in LDS and its sums go to
+// `partial`.  RAGGED: N is no multiple of a vector.  SUM: dsum is given.
+template <typename T, int K, bool SUB, bool RAGGED, bool SUM>
+__global__ void __launch_bounds__(1024) norm_grad_rows_kernel(const NormGradArgs a, int waves, int rows) {
+  constexpr int VEC = Vec<T>::N;
   typedef typename Vec<T>::Type V;
-  const int t = threadIdx.x % TPR, n = (int)a.N;
-  // (the row of a whole wave is a scalar: addresses are a scalar base and a lane's offset)
-  const int group = TPR >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : threadIdx.x / TPR;
+  __shared__ float meet[2][2][16];
+  extern __shared__ float joined[];   // [rows][threads of a row][VEC]
+  const RowOf<SUB> at(waves);
+  const int n = (int)a.N;
   const float inv_n = 1.0f / (float)n;
   float w[K][VEC], dw[K][VEC], db[K][VEC];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const Span at = span_of<VEC>(k * TPR + t, n);
-    if (a.w) load_params<T>(a.w, a.wide, at.first, w[k]);
+    const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
+    if (a.w) load_params<T>(a.w, a.wide, first, w[k]);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       if (!a.w) w[k][e] = 1.0f;
@@ -369,56 +434,56 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(const NormGradArg
     row = row < a.M ? row : a.M - 1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const Span at = span_of<VEC>(k * TPR + t, n);
-      r.dy[k] = load_vec((const T*)a.dy + row * a.lddy + at.first);
-      r.h[k] = load_vec((const T*)a.h + row * a.ldh + at.first);
+      const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
+      r.dy[k] = load_vec((const T*)a.dy + row * a.lddy + first);
+      r.h[k] = load_vec((const T*)a.h + row * a.ldh + first);
     }
     r.mean = a.mean[row];
     r.rstd = a.rstd[row];
   };
-  const int64_t stride = (int64_t)a.parts * ROWS;
-  int64_t first = (int64_t)blockIdx.x * ROWS;   // the workgroup's first row of this turn
+  const int64_t stride = (int64_t)a.parts * rows;
+  int64_t begin = (int64_t)blockIdx.x * rows;   // the workgroup's first row of this turn
   int turn = 0;
   // One turn: the next one's rows are on their way while this one's are summed, if registers
   // hold both.
   constexpr bool AHEAD = K <= 2;
   auto step = [&](Row& r, Row& next) -> bool {
-    const int64_t row = first + group;
-    const bool live = row < a.M, more = first + stride < a.M;
+    const int64_t row = begin + at.group;
+    const bool live = row < a.M, more = begin + stride < a.M;
     if (!AHEAD) fetch(r, row);
     V extra[SUM ? K : 1];
     if (SUM && live) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        extra[k] = load_vec((const T*)a.dsum + row * a.ldsum + span_of<VEC>(k * TPR + t, n).first);
+        extra[k] = load_vec((const T*)a.dsum + row * a.ldsum + span_of<VEC>(k * at.threads + at.lane, n).first);
     }
     if (AHEAD && more) fetch(next, row + stride);
-    float s1 = 0.0f, s2 = 0.0f;
+    float s[2] = {0.0f, 0.0f};   // of g = dy w and of g c, c = h - mean
     if (live) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const Span at = span_of<VEC>(k * TPR + t, n);
+        const Span span = span_of<VEC>(k * at.threads + at.lane, n);
         float t1 = 0.0f, t2 = 0.0f;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float d = (float)r.dy[k][e], c = (float)r.h[k][e] - r.mean, g = d * w[k][e];
           dw[k][e] += d * (c * r.rstd);
           db[k][e] += d;
-          t1 += RAGGED && e < at.twice ? 0.0f : g;
-          t2 += RAGGED && e < at.twice ? 0.0f : g * c;
+          t1 += RAGGED && e < span.twice ? 0.0f : g;
+          t2 += RAGGED && e < span.twice ? 0.0f : g * c;
         }
-        s1 += !RAGGED && at.twice ? 0.0f : t1;
-        s2 += !RAGGED && at.twice ? 0.0f : t2;
+        s[0] += !RAGGED && span.twice ? 0.0f : t1;
+        s[1] += !RAGGED && span.twice ? 0.0f : t2;
       }
     }
+    row_sums<SUB>(s, at, meet[turn]);
     // dx = rstd (g - mean(g) - xhat mean(g xhat)) with xhat = c rstd
-    const float shift = row_sum<TPR>(s1, meet[turn][0]) * inv_n * r.rstd;
-    const float slope = row_sum<TPR>(s2, meet[turn][1]) * inv_n * r.rstd * r.rstd;
+    const float shift = s[0] * inv_n * r.rstd, slope = s[1] * inv_n * r.rstd * r.rstd;
     if (live && a.dx) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const Span at = span_of<VEC>(k * TPR + t, n);
-        if (at.twice == VEC) continue;
+        const Span span = span_of<VEC>(k * at.threads + at.lane, n);
+        if (span.twice == VEC) continue;
         V out;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -428,16 +493,16 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(const NormGradArg
           if (SUM) d += (float)extra[k][e];
           out[e] = (T)d;
         }
-        store_vec((T*)a.dx + row * a.N + at.first, out);
+        store_vec((T*)a.dx + row * a.N + span.first, out);
       }
     }
-    first += stride;
+    begin += stride;
     turn ^= 1;
     return more;
   };
   Row one, other;
   if (AHEAD) {
-    fetch(one, first + group);
+    fetch(one, begin + at.group);
     while (step(one, other) && step(other, one)) {
     }
   } else {
@@ -448,72 +513,76 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(const NormGradArg
   float* sums = a.partial + (int64_t)blockIdx.x * 2 * n;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    if (ROWS == 1) {   // (of elements that two vectors have, both have the same sums)
-      const Span at = span_of<VEC>(k * TPR + t, n);
-      if (at.twice == VEC) continue;
+    if (rows == 1) {   // (of elements that two vectors have, both have the same sums)
+      const Span span = span_of<VEC>(k * at.threads + at.lane, n);
+      if (span.twice == VEC) continue;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        sums[at.first + e] = dw[k][e];
-        sums[n + at.first + e] = db[k][e];
+        sums[span.first + e] = dw[k][e];
+        sums[n + span.first + e] = db[k][e];
       }
       continue;
     }
+    const int width = at.threads * VEC;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) joined[group][t * VEC + e] = which == 0 ? dw[k][e] : db[k][e];
+      for (int e = 0; e < VEC; ++e) joined[at.group * width + at.lane * VEC + e] = which == 0 ? dw[k][e] : db[k][e];
       __syncthreads();
-      for (int c = threadIdx.x; c < TPR * VEC; c += BLOCK) {
-        const Span at = span_of<VEC>(k * TPR + c / VEC, n);
-        if (c % VEC < at.twice) continue;
+      for (int c = threadIdx.x; c < width; c += blockDim.x) {
+        const Span span = span_of<VEC>(k * at.threads + c / VEC, n);
+        if (c % VEC < span.twice) continue;
         float s = 0.0f;
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) s += joined[r][c];
-        sums[which * (int64_t)n + at.first + c % VEC] = s;
+        for (int r = 0; r < rows; ++r) s += joined[r * width + c];
+        sums[which * (int64_t)n + span.first + c % VEC] = s;
       }
     }
   }
 }
 
-// The workgroups' sums added up: 32 of the 2 N columns to a workgroup, 8 threads of 4 columns,
-// 32 of them taking every 32nd part.
+// The workgroups' sums added up: 32 of the 2 N columns to a workgroup, 16 threads to a column,
+// each taking every 16th part.
+constexpr int JOIN_COLUMNS = 32, JOIN_SLICES = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormGradArgs a) {
-  __shared__ float4 shared[32][8];
-  const int slice = threadIdx.x / 8, lane = threadIdx.x % 8;
-  const int64_t all = 2 * a.N, col = (block_number() * 8 + lane) * 4;
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+__global__ void __launch_bounds__(JOIN_COLUMNS* JOIN_SLICES) norm_grad_join_kernel(const NormGradArgs a) {
+  __shared__ float shared[JOIN_SLICES][JOIN_COLUMNS];
+  const int slice = threadIdx.x / JOIN_COLUMNS, lane = threadIdx.x % JOIN_COLUMNS;
+  const int64_t all = 2 * a.N, col = block_number() * JOIN_COLUMNS + lane;
+  float s = 0.0f;
   if (col < all) {
-    for (int part = slice; part < a.parts; part += 32) {
-      const float* p = a.partial + (int64_t)part * all + col;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < all) s[e] += p[e];
-    }
+    const float* p = a.partial + col;
+#pragma unroll 16
+    for (int part = slice; part < a.parts; part += JOIN_SLICES) s += p[(int64_t)part * all];
   }
-  shared[slice][lane] = float4{s[0], s[1], s[2], s[3]};
+  shared[slice][lane] = s;
   __syncthreads();
-  if (threadIdx.x >= 32) return;
-  const int64_t c = block_number() * 32 + threadIdx.x;
-  if (c >= all) return;
+  if (slice != 0 || col >= all) return;
   float total = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) total += ((const float*)&shared[i][0])[threadIdx.x];
-  void* out = c < a.N ? a.dw : a.db;
-  const int64_t i = c < a.N ? c : c - a.N;
+  for (int i = 0; i < JOIN_SLICES; ++i) total += shared[i][lane];
+  void* out = col < a.N ? a.dw : a.db;
+  const int64_t i = col < a.N ? col : col - a.N;
   if (!out) return;
   if (a.wide) ((float*)out)[i] = total; else ((T*)out)[i] = (T)total;
 }
 
-template <typename T, int TPR, int K, int BLOCK>
-int norm_grad_rows_launch(NormGradArgs a, hipStream_t stream) {
+template <typename T, int K, bool SUB>
+int norm_grad_rows_launch(NormGradArgs a, const RowPlan& plan, hipStream_t stream) {
   const bool params = a.dw || a.db;
-  const int64_t groups = ceil_div(a.M, BLOCK / TPR);
+  // as many rows at a time as 1024 threads hold, but all workgroups first
+  const int fit = SUB ? 64 : 16 / plan.waves;
+  const int64_t want = ceil_div(a.M, MOST_PARTS);
+  int rows = want < fit ? (int)want : fit;
+  if (SUB) rows = (rows + 3) / 4 * 4;   // (whole waves)
+  const int threads = SUB ? rows * 16 : plan.waves * rows * 64;
+  const int64_t groups = ceil_div(a.M, rows);
   a.parts = groups < MOST_PARTS ? (int)groups : MOST_PARTS;
   if (!params) a.partial = nullptr;
-#define AXN_NORM_GRAD(RAGGED, SUM)                                                                                   \
-  hipLaunchKernelGGL((norm_grad_rows_kernel<T, TPR, K, BLOCK, RAGGED, SUM>), dim3(a.parts), dim3(BLOCK), 0, stream, a)
+  const size_t lds = params && rows > 1 ? (size_t)threads * Vec<T>::N * sizeof(float) : 0;   // 32 KB at most
+#define AXN_NORM_GRAD(RAGGED, SUM)                                                                                 \
+  hipLaunchKernelGGL((norm_grad_rows_kernel<T, K, SUB, RAGGED, SUM>), dim3(a.parts), dim3(threads), lds, stream, a, \
+                     plan.waves, rows)
   const bool ragged = a.N % Vec<T>::N != 0;
   if (ragged && a.dsum) AXN_NORM_GRAD(true, true);
   if (ragged && !a.dsum) AXN_NORM_GRAD(true, false);
@@ -522,7 +591,8 @@ int norm_grad_rows_launch(NormGradArgs a, hipStream_t stream) {
 #undef AXN_NORM_GRAD
   AXN_HIP_TRY(hipGetLastError());
   if (params) {
-    hipLaunchKernelGGL(norm_grad_join_kernel<T>, grid_of(ceil_div(2 * a.N, 32)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(norm_grad_join_kernel<T>, grid_of(ceil_div(2 * a.N, JOIN_COLUMNS)),
+                       dim3(JOIN_COLUMNS * JOIN_SLICES), 0, stream, a);
     AXN_HIP_TRY(hipGetLastError());
   }
   return AXN_OK;
@@ -530,14 +600,10 @@ int norm_grad_rows_launch(NormGradArgs a, hipStream_t stream) {
 
 template <typename T>
 int norm_grad_rows(const NormGradArgs& a, hipStream_t stream) {
-  const int64_t v = ceil_div(a.N, Vec<T>::N);
-  if (v <= 32) return norm_grad_rows_launch<T, 16, 2, 256>(a, stream);
-  if (v <= 128) return norm_grad_rows_launch<T, 64, 2, 256>(a, stream);
-  if (v <= 256) return norm_grad_rows_launch<T, 128, 2, 1024>(a, stream);
-  if (v <= 512) return norm_grad_rows_launch<T, 256, 2, 1024>(a, stream);
-  if (v <= 1024) return norm_grad_rows_launch<T, 512, 2, 1024>(a, stream);
-  if (v <= 2048) return norm_grad_rows_launch<T, 1024, 2, 1024>(a, stream);
-  return norm_grad_rows_launch<T, 1024, 4, 1024>(a, stream);
+  const RowPlan plan = plan_row(a.N, Vec<T>::N);
+  if (plan.sub) return norm_grad_rows_launch<T, 2, true>(a, plan, stream);
+  if (plan.k == 2) return norm_grad_rows_launch<T, 2, false>(a, plan, stream);
+  return norm_grad_rows_launch<T, 4, false>(a, plan, stream);
 }
 
 template <int DT>
