@@ -30,6 +30,7 @@ __device__ __forceinline__ float param_at(const void* p, int wide, int64_t i) {
 }
 
 constexpr int ROW_THREADS = 256;
+constexpr int64_t kCached = 256 << 20;   // bytes that the memory-side cache holds
 constexpr int MOST_PARTS = 256;   // parts of the rows whose column sums meet in a second launch
 
 template <int THREADS>
@@ -166,13 +167,18 @@ struct Vec {
   static constexpr int N = 16 / sizeof(T);
   typedef T Type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
-template <typename T>
+// NT: not to be kept in the caches.
+template <bool NT = false, typename T>
 __device__ __forceinline__ typename Vec<T>::Type load_vec(const T* p) {
+  if (NT) return __builtin_nontemporal_load((const typename Vec<T>::Type*)p);
   return *(const typename Vec<T>::Type*)p;
 }
-template <typename T>
+template <bool NT = false, typename T>
 __device__ __forceinline__ void store_vec(T* p, typename Vec<T>::Type v) {
-  *(typename Vec<T>::Type*)p = v;
+  if (NT)
+    __builtin_nontemporal_store(v, (typename Vec<T>::Type*)p);
+  else
+    *(typename Vec<T>::Type*)p = v;
 }
 // VEC parameters from element i on, as floats.
 template <typename T>
@@ -257,15 +263,32 @@ __device__ __forceinline__ void row_sums(float (&x)[COUNT], const RowOf<SUB>& at
 }
 
 // RES: a residual is added.  RAGGED: N is no multiple of a vector.  A workgroup takes `rows` rows at
-// a time and goes on to those gridDim.x workgroups further; the parameters of its columns stay in
-// registers.
-template <typename T, int K, bool SUB, bool RES, bool RAGGED>
+// a time and goes on to those gridDim.x workgroups further, the parameters of its columns in
+// registers; ONCE: there is a workgroup for all rows, and nothing is kept in the caches.
+template <typename T, int K, bool SUB, bool RES, bool RAGGED, bool ONCE>
 __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int waves, int rows) {
   constexpr int VEC = Vec<T>::N;
   typedef typename Vec<T>::Type V;
   __shared__ float shared[2][2][16];
   const RowOf<SUB> at(waves);
   const int n = (int)a.N;
+  struct Row {
+    V x[K], r[RES ? K : 1];
+  };
+  auto fetch = [&](Row& f, int64_t row) {   // (behind the last row: that row again)
+    row = row < a.M ? row : a.M - 1;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
+      f.x[k] = load_vec<ONCE>((const T*)a.x + row * a.ldx + first);
+      if (RES) f.r[k] = load_vec<ONCE>((const T*)a.r + row * a.ldr + first);
+    }
+  };
+  const int64_t stride = (int64_t)gridDim.x * rows;
+  int64_t begin = (int64_t)blockIdx.x * rows;   // the workgroup's first row of this turn
+  constexpr bool AHEAD = K <= 2 && !ONCE;
+  Row one, other;
+  if (AHEAD || ONCE) fetch(one, begin + at.group);
   float w[K][VEC], b[K][VEC];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -278,26 +301,13 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
       if (!a.b) b[k][e] = 0.0f;
     }
   }
-  struct Row {
-    V x[K], r[RES ? K : 1];
-  };
-  auto fetch = [&](Row& f, int64_t row) {   // (behind the last row: that row again)
-    row = row < a.M ? row : a.M - 1;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
-      f.x[k] = load_vec((const T*)a.x + row * a.ldx + first);
-      if (RES) f.r[k] = load_vec((const T*)a.r + row * a.ldr + first);
-    }
-  };
-  const int64_t stride = (int64_t)gridDim.x * rows;
-  int64_t begin = (int64_t)blockIdx.x * rows;   // the workgroup's first row of this turn
   int turn = 0;
-  constexpr bool AHEAD = K <= 2;
+  // One turn: the next one's rows are on their way while this one's are summed, if registers
+  // hold both.
   auto step = [&](Row& f, Row& next) -> bool {
     const int64_t row = begin + at.group;
-    const bool live = row < a.M, more = begin + stride < a.M;
-    if (!AHEAD) fetch(f, row);
+    const bool live = row < a.M, more = !ONCE && begin + stride < a.M;
+    if (!AHEAD && !ONCE) fetch(f, row);
     if (AHEAD && more) fetch(next, row + stride);
     float h[K][VEC], s[1] = {0.0f};
 #pragma unroll
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
       if (RES) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) f.x[k][e] = (T)((float)f.x[k][e] + (float)f.r[k][e]);
-        if (live && span.twice < VEC) store_vec((T*)a.h + row * a.N + span.first, f.x[k]);
+        if (live && span.twice < VEC) store_vec<ONCE>((T*)a.h + row * a.N + span.first, f.x[k]);
       }
       float t = 0.0f;
 #pragma unroll
@@ -340,7 +350,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
         V y;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) y[e] = (T)(h[k][e] * rstd * w[k][e] + b[k][e]);
-        store_vec((T*)a.y + row * a.N + span.first, y);
+        store_vec<ONCE>((T*)a.y + row * a.N + span.first, y);
       }
       if (at.lane == 0 && a.mean) {
         a.mean[row] = mean;
@@ -351,9 +361,9 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
     turn ^= 1;
     return more;
   };
-  Row one, other;
-  if (AHEAD) {
-    fetch(one, begin + at.group);
+  if (ONCE) {
+    step(one, one);
+  } else if (AHEAD) {
     while (step(one, other) && step(other, one)) {
     }
   } else {
@@ -378,17 +388,21 @@ template <typename T, int K, bool SUB>
 int norm_rows_launch(const NormArgs& a, const RowPlan& plan, hipStream_t stream) {
   const int rows = SUB ? 16 : plan.waves >= 4 ? 1 : 4 / plan.waves;
   const int threads = SUB ? 256 : plan.waves * rows * 64;
+  const bool once = a.r && 4 * a.M * a.N * (int64_t)sizeof(T) > kCached;
   int64_t groups = ceil_div(a.M, rows);
   const int64_t most = 256 * (2048 / threads) / 2;
-  if (groups > most) groups = most;
-#define AXN_NORM(RES, RAGGED)                                                                              \
-  hipLaunchKernelGGL((norm_rows_kernel<T, K, SUB, RES, RAGGED>), dim3((unsigned)groups), dim3(threads), 0, \
-                     stream, a, plan.waves, rows)
+  if (!once && groups > most) groups = most;
   const bool ragged = a.N % Vec<T>::N != 0;
-  if (ragged && a.r) AXN_NORM(true, true);
-  if (ragged && !a.r) AXN_NORM(false, true);
-  if (!ragged && a.r) AXN_NORM(true, false);
-  if (!ragged && !a.r) AXN_NORM(false, false);
+#define AXN_NORM(RES, RAGGED, ONCE)                                                                              \
+  if ((a.r != nullptr) == RES && ragged == RAGGED && once == ONCE)                                               \
+  hipLaunchKernelGGL((norm_rows_kernel<T, K, SUB, RES, RAGGED, ONCE>), dim3((unsigned)groups), dim3(threads), 0, \
+                     stream, a, plan.waves, rows)
+  AXN_NORM(false, false, false);
+  AXN_NORM(false, true, false);
+  AXN_NORM(true, false, false);
+  AXN_NORM(true, false, true);
+  AXN_NORM(true, true, false);
+  AXN_NORM(true, true, true);
 #undef AXN_NORM
   AXN_HIP_TRY(hipGetLastError());
   return AXN_OK;
@@ -411,21 +425,10 @@ __global__ void __launch_bounds__(1024) norm_grad_rows_kernel(const NormGradArgs
   constexpr int VEC = Vec<T>::N;
   typedef typename Vec<T>::Type V;
   __shared__ float meet[2][2][16];
-  extern __shared__ float joined[];   // [rows][threads of a row][VEC]
+  extern __shared__ __align__(16) float joined[];   // [rows][dw, db][vectors of a row][VEC]
   const RowOf<SUB> at(waves);
   const int n = (int)a.N;
   const float inv_n = 1.0f / (float)n;
-  float w[K][VEC], dw[K][VEC], db[K][VEC];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
-    if (a.w) load_params<T>(a.w, a.wide, first, w[k]);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (!a.w) w[k][e] = 1.0f;
-      dw[k][e] = db[k][e] = 0.0f;
-    }
-  }
   struct Row {
     V dy[K], h[K];
     float mean, rstd;
@@ -443,10 +446,23 @@ __global__ void __launch_bounds__(1024) norm_grad_rows_kernel(const NormGradArgs
   };
   const int64_t stride = (int64_t)a.parts * rows;
   int64_t begin = (int64_t)blockIdx.x * rows;   // the workgroup's first row of this turn
+  constexpr bool AHEAD = K <= 2;
+  Row one, other;
+  if (AHEAD) fetch(one, begin + at.group);
+  float w[K][VEC], dw[K][VEC], db[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
+    if (a.w) load_params<T>(a.w, a.wide, first, w[k]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (!a.w) w[k][e] = 1.0f;
+      dw[k][e] = db[k][e] = 0.0f;
+    }
+  }
   int turn = 0;
   // One turn: the next one's rows are on their way while this one's are summed, if registers
   // hold both.
-  constexpr bool AHEAD = K <= 2;
   auto step = [&](Row& r, Row& next) -> bool {
     const int64_t row = begin + at.group;
     const bool live = row < a.M, more = begin + stride < a.M;
@@ -500,9 +516,7 @@ __global__ void __launch_bounds__(1024) norm_grad_rows_kernel(const NormGradArgs
     turn ^= 1;
     return more;
   };
-  Row one, other;
   if (AHEAD) {
-    fetch(one, begin + at.group);
     while (step(one, other) && step(other, one)) {
     }
   } else {
@@ -511,33 +525,37 @@ __global__ void __launch_bounds__(1024) norm_grad_rows_kernel(const NormGradArgs
   }
   if (!a.partial) return;
   float* sums = a.partial + (int64_t)blockIdx.x * 2 * n;
+  if (rows == 1) {   // (of elements that two vectors have, both have the same sums)
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (rows == 1) {   // (of elements that two vectors have, both have the same sums)
+    for (int k = 0; k < K; ++k) {
       const Span span = span_of<VEC>(k * at.threads + at.lane, n);
       if (span.twice == VEC) continue;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        sums[span.first + e] = dw[k][e];
-        sums[n + span.first + e] = db[k][e];
-      }
-      continue;
-    }
-    const int width = at.threads * VEC;
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) joined[at.group * width + at.lane * VEC + e] = which == 0 ? dw[k][e] : db[k][e];
-      __syncthreads();
-      for (int c = threadIdx.x; c < width; c += blockDim.x) {
-        const Span span = span_of<VEC>(k * at.threads + c / VEC, n);
-        if (c % VEC < span.twice) continue;
-        float s = 0.0f;
-        for (int r = 0; r < rows; ++r) s += joined[r * width + c];
-        sums[which * (int64_t)n + span.first + c % VEC] = s;
+      for (int e = 0; e < VEC; e += 4) {
+        store_vec(sums + span.first + e, Vec<float>::Type{dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]});
+        store_vec(sums + n + span.first + e, Vec<float>::Type{db[k][e], db[k][e + 1], db[k][e + 2], db[k][e + 3]});
       }
     }
+    return;
+  }
+  const int width = K * at.threads * VEC;   // of a row, vectors behind its end included
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float* mine = joined + at.group * 2 * width + (k * at.threads + at.lane) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      *(float4*)(mine + e) = float4{dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]};
+      *(float4*)(mine + width + e) = float4{db[k][e], db[k][e + 1], db[k][e + 2], db[k][e + 3]};
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
+    const int place = c < width ? c : c - width;
+    const Span span = span_of<VEC>(place / VEC, n);
+    if (place % VEC < span.twice) continue;
+    float s = 0.0f;
+    for (int r = 0; r < rows; ++r) s += joined[r * 2 * width + c];
+    sums[(c < width ? 0 : n) + span.first + place % VEC] = s;
   }
 }
 
@@ -579,10 +597,18 @@ int norm_grad_rows_launch(NormGradArgs a, const RowPlan& plan, hipStream_t strea
   const int64_t groups = ceil_div(a.M, rows);
   a.parts = groups < MOST_PARTS ? (int)groups : MOST_PARTS;
   if (!params) a.partial = nullptr;
-  const size_t lds = params && rows > 1 ? (size_t)threads * Vec<T>::N * sizeof(float) : 0;   // 32 KB at most
-#define AXN_NORM_GRAD(RAGGED, SUM)                                                                                 \
-  hipLaunchKernelGGL((norm_grad_rows_kernel<T, K, SUB, RAGGED, SUM>), dim3(a.parts), dim3(threads), lds, stream, a, \
-                     plan.waves, rows)
+  const size_t lds = params && rows > 1 ? (size_t)threads * 2 * K * Vec<T>::N * sizeof(float) : 0;
+  constexpr size_t MOST_LDS = 1024 * 2 * K * Vec<T>::N * sizeof(float);
+#define AXN_NORM_GRAD(RAGGED, SUM)                                                                                  \
+  do {                                                                                                              \
+    static std::atomic<unsigned long long> allowed{0};                                                              \
+    if (lds > 32768) {                                                                                              \
+      const int rc = allow_lds((const void*)norm_grad_rows_kernel<T, K, SUB, RAGGED, SUM>, MOST_LDS, allowed);      \
+      if (rc) return rc;                                                                                            \
+    }                                                                                                               \
+    hipLaunchKernelGGL((norm_grad_rows_kernel<T, K, SUB, RAGGED, SUM>), dim3(a.parts), dim3(threads), lds, stream,  \
+                       a, plan.waves, rows);                                                                        \
+  } while (0)
   const bool ragged = a.N % Vec<T>::N != 0;
   if (ragged && a.dsum) AXN_NORM_GRAD(true, true);
   if (ragged && !a.dsum) AXN_NORM_GRAD(true, false);
@@ -618,7 +644,7 @@ int norm_launch(const NormArgs& a, hipStream_t stream) {
 template <int DT>
 int norm_grad_launch(const NormGradArgs& a, hipStream_t stream) {
   typedef typename Elem<DT>::type T;
-  if (a.M > 0 && a.N >= Vec<T>::N && a.N <= 16384) return norm_grad_rows<T>(a, stream);
+  if (a.M > 0 && a.N >= Vec<T>::N && a.N <= 4096 * Vec<T>::N) return norm_grad_rows<T>(a, stream);
   if (a.dx) {
     hipLaunchKernelGGL(norm_dx_any_kernel<T>, grid_of(a.M), dim3(ROW_THREADS), 0, stream, a);
     AXN_HIP_TRY(hipGetLastError());
