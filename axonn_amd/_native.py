@@ -138,7 +138,7 @@ EXT_SYMBOLS = {
 
 _lib = None
 _probe_lib = None
-# axn_fast.so (csrc/fast.cpp): the host side of the usual Linear calls, same kernels.  None before `load` and where it is
+# axn_fast.so (csrc/fast.cpp): the host side of the usual Linear, layer norm and AdamW calls, same kernels.  None before `load` and where it is
 # not built or does not fit: every caller then goes the general way, which it also goes where a function of `fast` answers
 # None.
 fast = None
@@ -171,10 +171,12 @@ def _load_fast(lib):
         loader = importlib.machinery.ExtensionFileLoader("axn_fast", path)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("axn_fast", loader))
         loader.exec_module(module)
-        built, wanted = (module.ABI_VERSION, module.BUILT_FOR), (ABI_VERSION, fast_built_for(torch))
+        built = module.ABI_VERSION, getattr(module, "EXT_ABI_VERSION", None), module.BUILT_FOR
+        wanted = ABI_VERSION, EXT_ABI_VERSION, fast_built_for(torch)
         if built != wanted:
             raise ImportError("it was built for %s, this is %s" % (built, wanted))
         module.bind(dict({name: ctypes.cast(getattr(lib, name), _vp).value for name in module.entry_points()}, check=check))
+        module.bind_ext({name: ctypes.cast(getattr(lib, name), _vp).value for name in module.ext_entry_points()})
     except (ImportError, AttributeError) as error:
         warnings.warn("axn_fast.so is not used, Linear calls take more host time (%s); run "
                       "`python -m axonn_amd.csrc.build`" % error, stacklevel=3)

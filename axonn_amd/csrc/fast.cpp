@@ -1,5 +1,5 @@
-// The usual calls of a Linear layer without their way through Python: checks, output and workspace tensors and
-// the library's entry point in one function each.  Whatever is not usual - another layout, type, device or
+// The usual calls of a Linear layer, of a layer norm and of AdamW's step without their way through Python: checks, output
+// and workspace tensors and the library's entry point in one function each.  Whatever is not usual - another layout, type, device or
 // alignment, an empty batch, a size that needs padding, a mode that watches tensors - answers None before anything is
 // launched, and the caller (axonn_amd/ops.py, fully_connected.py) goes the general way from the start.  An error of the
 // library is raised, as it is there: it can follow a launch (one that an earlier call left behind is reported by the
@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "axn.h"
+#include "axn_ext.h"
 
 namespace {
 
@@ -39,6 +40,13 @@ struct Library {
   ENTRY_POINTS(DECLARE)
 #undef DECLARE
 } lib;
+#define EXT_ENTRY_POINTS(X) \
+  X(axn_layer_norm_fwd) X(axn_layer_norm_bwd) X(axn_layer_norm_bwd_workspace_bytes) X(axn_mt_adamw) X(axn_mt_adamw8)
+struct ExtLibrary {   // (bound by a call of their own, as their header has a version of its own)
+#define DECLARE(name) decltype(&::name) name = nullptr;
+  EXT_ENTRY_POINTS(DECLARE)
+#undef DECLARE
+} ext;
 PyObject* check_status = nullptr;   // axonn_amd._native.check: raises the library's error
 
 // Rows further apart are packed first by the general way.
@@ -347,6 +355,169 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- layer norm ----------------------------------------------------------------------------
+bool known(at::ScalarType t) { return is16(t) || t == at::kFloat; }
+// Rows of a type the kernels take, dense; `like`: of its type and size too.
+bool dense_rows(const at::Tensor& t, c10::DeviceIndex device, const at::Tensor* like = nullptr) {
+  return plain(t, device) && t.dim() == 2 && known(t.scalar_type()) && t.size(0) >= 1 && t.size(1) >= 1 &&
+         t.size(0) <= 0x7fffffff && t.size(1) <= 0x7fffffff &&
+         (like == nullptr || (t.scalar_type() == like->scalar_type() && t.sizes() == like->sizes()));
+}
+bool norm_param(const at::Tensor& t, const at::Tensor& rows, c10::DeviceIndex device) {
+  return plain(t, device) && t.dim() == 1 && t.size(0) == rows.size(1) &&
+         (t.scalar_type() == rows.scalar_type() || t.scalar_type() == at::kFloat);
+}
+
+// layer_norm_fwd(x, weight, bias, eps, residual, save) -> (y, h, mean, rstd) or None
+PyObject* layer_norm_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !THPVariable_CheckExact(args[0]) || !is_tensor_or_none(args[1]) || !is_tensor_or_none(args[2]) ||
+      !PyFloat_CheckExact(args[3]) || !is_tensor_or_none(args[4]) || ext.axn_layer_norm_fwd == nullptr)
+    Py_RETURN_NONE;
+  const at::Tensor x = THPVariable_Unpack(args[0]), w = tensor_or_none(args[1]), b = tensor_or_none(args[2]),
+                   r = tensor_or_none(args[4]);
+  const double eps = PyFloat_AS_DOUBLE(args[3]);
+  const bool save = truth(args[5]);
+  const c10::DeviceIndex device = current_device_for(x);
+  if (!dense_rows(x, device) || !nothing_watches() || (r.defined() && !dense_rows(r, device, &x)) ||
+      (w.defined() && !norm_param(w, x, device)) || (b.defined() && !norm_param(b, x, device)) ||
+      (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()))
+    Py_RETURN_NONE;
+  const int64_t M = x.size(0), N = x.size(1);
+  const at::ScalarType type = x.scalar_type(), param = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : type;
+  at::Tensor y, h, mean, rstd;
+  int status;
+  {
+    Unlocked unlocked;
+    y = empty({M, N}, type, x);
+    if (r.defined()) h = empty({M, N}, type, x);
+    if (save) {
+      mean = empty({M}, at::kFloat, x);
+      rstd = empty({M}, at::kFloat, x);
+    }
+    status = ext.axn_layer_norm_fwd(pointer(x), pointer(r), pointer(w), pointer(b), pointer(y), pointer(h),
+                                    (float*)pointer(mean), (float*)pointer(rstd), code_of(type), code_of(param), M, N, N, N,
+                                    (float)eps, c10::hip::getCurrentHIPStream(device).stream());
+  }
+  if (status != AXN_OK) return no_result(status);
+  PyObject* out = PyTuple_New(4);
+  PyTuple_SET_ITEM(out, 0, wrap(y));
+  PyTuple_SET_ITEM(out, 1, wrap(h));
+  PyTuple_SET_ITEM(out, 2, wrap(mean));
+  PyTuple_SET_ITEM(out, 3, wrap(rstd));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_norm_bwd(dy, h, weight, mean, rstd, dsum, want_dx, want_dweight, want_dbias) -> (dx, dweight, dbias) or None
+PyObject* layer_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || ext.axn_layer_norm_bwd == nullptr || !is_tensor_or_none(args[5])) Py_RETURN_NONE;
+  for (int i = 0; i < 5; ++i)   // (without a weight: the general way, which is told the parameters' type)
+    if (!THPVariable_CheckExact(args[i])) Py_RETURN_NONE;
+  const at::Tensor dy = THPVariable_Unpack(args[0]), h = THPVariable_Unpack(args[1]), w = THPVariable_Unpack(args[2]),
+                   mean = THPVariable_Unpack(args[3]), rstd = THPVariable_Unpack(args[4]), ds = tensor_or_none(args[5]);
+  const bool want_dx = truth(args[6]), want_dw = truth(args[7]), want_db = truth(args[8]);
+  const c10::DeviceIndex device = current_device_for(dy);
+  if (!(want_dx || want_dw || want_db) || !dense_rows(dy, device) || !dense_rows(h, device, &dy) || !norm_param(w, dy, device) ||
+      (ds.defined() && !dense_rows(ds, device, &dy)) || !nothing_watches())
+    Py_RETURN_NONE;
+  const int64_t M = dy.size(0), N = dy.size(1);
+  for (const at::Tensor* t : {&mean, &rstd})
+    if (!t->is_cuda() || t->get_device() != device || t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != M ||
+        !t->is_contiguous())
+      Py_RETURN_NONE;
+  const at::ScalarType type = dy.scalar_type(), param = w.scalar_type();
+  at::Tensor dx, dw, db;
+  int status;
+  {
+    Unlocked unlocked;
+    if (want_dx) dx = empty({M, N}, type, dy);
+    if (want_dw) dw = empty({N}, param, dy);
+    if (want_db) db = empty({N}, param, dy);
+    const Workspace ws(want_dw || want_db ? ext.axn_layer_norm_bwd_workspace_bytes(M, N) : 0, dy);
+    status = ext.axn_layer_norm_bwd(pointer(dy), pointer(h), pointer(w), (const float*)pointer(mean),
+                                    (const float*)pointer(rstd), pointer(ds), pointer(dx), pointer(dw), pointer(db),
+                                    code_of(type), code_of(param), M, N, N, N, N, ws.at, ws.bytes,
+                                    c10::hip::getCurrentHIPStream(device).stream());
+  }
+  if (status != AXN_OK) return no_result(status);
+  PyObject* out = PyTuple_New(3);
+  PyTuple_SET_ITEM(out, 0, wrap(dx));
+  PyTuple_SET_ITEM(out, 1, wrap(dw));
+  PyTuple_SET_ITEM(out, 2, wrap(db));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- AdamW ---------------------------------------------------------------------------------
+// The pointers of a list of dense tensors of one type on the current device, and their sizes into
+// `sizes` if that is empty; a size of its own for each is else in `expected`.
+struct TensorList {
+  std::vector<void*> at;
+  at::ScalarType type = at::ScalarType::Undefined;
+  bool take(PyObject* list, Py_ssize_t n, c10::DeviceIndex device, std::vector<int64_t>* sizes, int64_t per, int64_t unit) {
+    if (!PyList_CheckExact(list) || PyList_GET_SIZE(list) != n) return false;
+    const bool first = sizes->empty();
+    at.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* o = PyList_GET_ITEM(list, i);
+      if (!THPVariable_CheckExact(o)) return false;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.is_neg() || t.is_conj()) return false;
+      if (i == 0) type = t.scalar_type();
+      if (t.scalar_type() != type) return false;
+      if (first) sizes->push_back(t.numel());
+      else if (t.numel() != ((*sizes)[i] + unit - 1) / unit * per) return false;
+      at.push_back(const_cast<void*>(t.const_data_ptr()));
+    }
+    return true;
+  }
+};
+
+// adamw(grads, params32, exp_avg or codes, exp_avg_sq or exponents, params_lowp or None, address of the hparams, inv_scale,
+//       scan's address or None, seed or None) -> True, or None; the lists are not empty
+PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9 || ext.axn_mt_adamw == nullptr || !PyList_CheckExact(args[0]) || PyList_GET_SIZE(args[0]) == 0 ||
+      !PyLong_CheckExact(args[5]) || !PyFloat_CheckExact(args[6]) || !(args[7] == Py_None || PyLong_CheckExact(args[7])) ||
+      !(args[8] == Py_None || PyLong_CheckExact(args[8])) || !nothing_watches())
+    Py_RETURN_NONE;
+  const bool eight = args[8] != Py_None;
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  const c10::DeviceIndex device = c10::hip::current_device();
+  std::vector<int64_t> sizes;
+  sizes.reserve(n);
+  TensorList g, p, m, v, low;
+  const bool copy = args[4] != Py_None;
+  if (!g.take(args[0], n, device, &sizes, 1, 1) || !p.take(args[1], n, device, &sizes, 1, 1) ||
+      !m.take(args[2], n, device, &sizes, eight ? 2 * AXN_ADAMW8_BLOCK : 1, eight ? AXN_ADAMW8_BLOCK : 1) ||
+      !v.take(args[3], n, device, &sizes, eight ? 2 : 1, eight ? AXN_ADAMW8_BLOCK : 1) ||
+      (copy && !low.take(args[4], n, device, &sizes, 1, 1)))
+    Py_RETURN_NONE;
+  const at::ScalarType state = eight ? at::kByte : at::kFloat;
+  if (!known(g.type) || p.type != at::kFloat || m.type != state || v.type != state || (copy && !is16(low.type))) Py_RETURN_NONE;
+  const auto* hp = (const axn_adamw_hparams*)PyLong_AsVoidPtr(args[5]);
+  const float inv_scale = (float)PyFloat_AS_DOUBLE(args[6]);
+  const auto* scan = args[7] == Py_None ? nullptr : (const axn_scan_result*)PyLong_AsVoidPtr(args[7]);
+  const uint64_t seed = eight ? PyLong_AsUnsignedLongLongMask(args[8]) : 0;
+  if (PyErr_Occurred()) return nullptr;
+  int status;
+  {
+    Unlocked unlocked;
+    const auto stream = c10::hip::getCurrentHIPStream(device).stream();
+    void* const* plow = copy ? low.at.data() : nullptr;
+    const int gdt = code_of(g.type), pdt = copy ? code_of(low.type) : AXN_BF16;
+    status = eight ? ext.axn_mt_adamw8(g.at.data(), p.at.data(), m.at.data(), v.at.data(), plow, sizes.data(), n, gdt, pdt,
+                                       inv_scale, seed, scan, hp, stream)
+                   : ext.axn_mt_adamw(g.at.data(), p.at.data(), m.at.data(), v.at.data(), plow, sizes.data(), n, gdt, pdt,
+                                      inv_scale, scan, hp, stream);
+  }
+  if (status != AXN_OK) return no_result(status);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address, "check": axonn_amd._native.check}): the library's entry points, and what raises their errors
 PyObject* bind(PyObject*, PyObject* table) {
   Library bound;
@@ -359,12 +530,19 @@ PyObject* bind(PyObject*, PyObject* table) {
     if (PyErr_Occurred()) return nullptr;                                                 \
   }
   ENTRY_POINTS(BIND)
-#undef BIND
   PyObject* check = PyMapping_GetItemString(table, "check");
   if (check == nullptr) return nullptr;
   Py_XDECREF(check_status);
   check_status = check;
   lib = bound;
+  Py_RETURN_NONE;
+}
+// bind_ext({name: address}): those of axn_ext.h
+PyObject* bind_ext(PyObject*, PyObject* table) {
+  ExtLibrary bound;
+  EXT_ENTRY_POINTS(BIND)
+#undef BIND
+  ext = bound;
   Py_RETURN_NONE;
 }
 PyObject* entry_points(PyObject*, PyObject*) {
@@ -376,6 +554,11 @@ PyObject* entry_points(PyObject*, PyObject*) {
     Py_DECREF(s);                                         \
   }
   ENTRY_POINTS(NAME)
+  return names;
+}
+PyObject* ext_entry_points(PyObject*, PyObject*) {
+  PyObject* names = PyList_New(0);
+  EXT_ENTRY_POINTS(NAME)
 #undef NAME
   return names;
 }
@@ -384,7 +567,12 @@ PyMethodDef methods[] = {
     {"gemm_fwd", (PyCFunction)(void (*)(void))gemm_fwd, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr},
     {"backward", (PyCFunction)(void (*)(void))backward, METH_FASTCALL, nullptr},
+    {"layer_norm_fwd", (PyCFunction)(void (*)(void))layer_norm_fwd, METH_FASTCALL, nullptr},
+    {"layer_norm_bwd", (PyCFunction)(void (*)(void))layer_norm_bwd, METH_FASTCALL, nullptr},
+    {"adamw", (PyCFunction)(void (*)(void))adamw, METH_FASTCALL, nullptr},
     {"bind", bind, METH_O, nullptr},
+    {"bind_ext", bind_ext, METH_O, nullptr},
+    {"ext_entry_points", ext_entry_points, METH_NOARGS, nullptr},
     {"entry_points", entry_points, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
@@ -395,6 +583,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "axn_fast", nullptr, -1, methods};
 PyMODINIT_FUNC PyInit_axn_fast() {
   PyObject* m = PyModule_Create(&module);
   if (m != nullptr && (PyModule_AddIntConstant(m, "ABI_VERSION", AXN_ABI_VERSION) != 0 ||
+                       PyModule_AddIntConstant(m, "EXT_ABI_VERSION", AXN_EXT_ABI_VERSION) != 0 ||
                        PyModule_AddStringConstant(m, "BUILT_FOR", AXN_BUILT_FOR) != 0)) {
     Py_DECREF(m);
     return nullptr;

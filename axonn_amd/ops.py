@@ -7,6 +7,7 @@ torch op: tensors that are not on a GPU are rejected.
 """
 
 import contextlib
+import ctypes
 import functools
 
 import torch
@@ -794,6 +795,10 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, residual=None, save=True
     """(h - mean) rstd weight + bias over the last dimension of h = x, or of h = x + residual rounded to their type.
     x [M, N] of bf16, fp16 or fp32, weight and bias [N] of that type or fp32.  Returns (y, h, mean, rstd): h is None
     without a residual, mean and rstd (fp32 [M], what `layer_norm_bwd` needs) are None unless `save`."""
+    if nv.fast is not None:
+        done = nv.fast.layer_norm_fwd(x, weight, bias, eps, residual, save)
+        if done is not None:
+            return done
     name = "layer_norm_fwd"
     where = _device_of(name, x, weight, bias, residual)
     code = nv.dtype_code(x.dtype)
@@ -829,6 +834,10 @@ def layer_norm_bwd(dy, h, weight, mean, rstd, dsum=None, want_dx=True, want_dwei
     """Gradients of `layer_norm_fwd` for dy [M, N], h its normalised rows (x, or the sum) and their statistics: (dx,
     dweight, dbias), None for what is not wanted.  dsum is the gradient that reaches the sum from elsewhere; dx is then
     that of x and of the residual.  dweight and dbias are of weight's type (`param_dtype` without one: the rows')."""
+    if nv.fast is not None:
+        done = nv.fast.layer_norm_bwd(dy, h, weight, mean, rstd, dsum, want_dx, want_dweight, want_dbias)
+        if done is not None:
+            return done
     name = "layer_norm_bwd"
     where = _device_of(name, dy, h, weight, mean, rstd, dsum)
     code = nv.dtype_code(dy.dtype)
@@ -1024,6 +1033,14 @@ def _step_lists(name, grads, params32, params_lowp, *state):
     return nv.dtype_code(grads[0].dtype), nv.BF16 if params_lowp is None else nv.dtype_code(params_lowp[0].dtype)
 
 
+def _step_in_one_call(grads, params32, m, v, params_lowp, hparams, inv_scale, scan, seed):
+    """The step through `fast`; false for lists that are not as usual, which take the checks that follow."""
+    if nv.fast is None or type(hparams) is not nv.AdamWHParams or (scan is not None and scan.buf.device != grads[0].device):
+        return False
+    return nv.fast.adamw(grads, params32, m, v, params_lowp, ctypes.addressof(hparams), float(inv_scale),
+                         None if scan is None else scan.ptr(), seed) is not None
+
+
 def adamw_hparams(step, lr, beta1, beta2, eps, weight_decay):
     """Host-side scalars of AdamW step number `step` (1-based), in Python doubles as `adam_hparams`."""
     return nv.AdamWHParams(
@@ -1042,7 +1059,7 @@ def mt_adamw(grads, params32, exp_avg, exp_avg_sq, params_lowp, hparams, inv_sca
     moments, `params_lowp` a bf16 or fp16 copy of the weights or None; hparams from `adamw_hparams`; scan from `mt_scan`
     clips, and skips the whole step on the device after an overflow."""
     name = "mt_adamw"
-    if len(grads) == 0:
+    if len(grads) == 0 or _step_in_one_call(grads, params32, exp_avg, exp_avg_sq, params_lowp, hparams, inv_scale, scan, None):
         return
     gdt, pdt = _step_lists(name, grads, params32, params_lowp, exp_avg, exp_avg_sq)
     for what, moments in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)):
@@ -1079,7 +1096,7 @@ def mt_adamw8(grads, params32, codes, exponents, params_lowp, hparams, seed, inv
     its exponents, from `adamw8_state`.  `seed` (64 bits) makes the random words of the rounding: another one for every
     step; equal calls give equal bits."""
     name = "mt_adamw8"
-    if len(grads) == 0:
+    if len(grads) == 0 or _step_in_one_call(grads, params32, codes, exponents, params_lowp, hparams, inv_scale, scan, seed):
         return
     gdt, pdt = _step_lists(name, grads, params32, params_lowp, codes, exponents)
     for g, c, e in zip(grads, codes, exponents):
