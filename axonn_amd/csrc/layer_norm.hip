@@ -372,14 +372,16 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
   }
 }
 
-// Waves and vectors of a lane for rows of N elements, and whether 16 lanes do.
+// Waves and vectors of a lane for rows of N elements, and whether 16 lanes do.  `single`: one vector
+// to a lane as long as 16 waves hold the row.
 struct RowPlan {
   int k, waves;
   bool sub;
 };
-inline RowPlan plan_row(int64_t N, int vec) {
+inline RowPlan plan_row(int64_t N, int vec, bool single) {
   const int64_t v = ceil_div(N, vec);
-  if (v <= 32) return {2, 1, true};
+  if (v <= 32) return {v <= 16 ? 1 : 2, 1, true};
+  if (single && v <= 1024) return {1, (int)ceil_div(v, 64), false};
   if (v <= 2048) return {2, (int)ceil_div(v, 128), false};
   return {4, (int)ceil_div(v, 256), false};
 }
@@ -410,8 +412,8 @@ int norm_rows_launch(const NormArgs& a, const RowPlan& plan, hipStream_t stream)
 
 template <typename T>
 int norm_rows(const NormArgs& a, hipStream_t stream) {
-  const RowPlan plan = plan_row(a.N, Vec<T>::N);
-  if (plan.sub) return norm_rows_launch<T, 2, true>(a, plan, stream);
+  const RowPlan plan = plan_row(a.N, Vec<T>::N, false);
+  if (plan.sub) return plan.k == 1 ? norm_rows_launch<T, 1, true>(a, plan, stream) : norm_rows_launch<T, 2, true>(a, plan, stream);
   if (plan.k == 2) return norm_rows_launch<T, 2, false>(a, plan, stream);
   return norm_rows_launch<T, 4, false>(a, plan, stream);
 }
@@ -626,8 +628,10 @@ int norm_grad_rows_launch(NormGradArgs a, const RowPlan& plan, hipStream_t strea
 
 template <typename T>
 int norm_grad_rows(const NormGradArgs& a, hipStream_t stream) {
-  const RowPlan plan = plan_row(a.N, Vec<T>::N);
-  if (plan.sub) return norm_grad_rows_launch<T, 2, true>(a, plan, stream);
+  const RowPlan plan = plan_row(a.N, Vec<T>::N, true);
+  if (plan.sub)
+    return plan.k == 1 ? norm_grad_rows_launch<T, 1, true>(a, plan, stream) : norm_grad_rows_launch<T, 2, true>(a, plan, stream);
+  if (plan.k == 1) return norm_grad_rows_launch<T, 1, false>(a, plan, stream);
   if (plan.k == 2) return norm_grad_rows_launch<T, 2, false>(a, plan, stream);
   return norm_grad_rows_launch<T, 4, false>(a, plan, stream);
 }
