@@ -264,8 +264,8 @@ __device__ __forceinline__ void row_sums(float (&x)[COUNT], const RowOf<SUB>& at
 
 // RES: a residual is added.  RAGGED: N is no multiple of a vector.  A workgroup takes `rows` rows at
 // a time and goes on to those gridDim.x workgroups further, the parameters of its columns in
-// registers; ONCE: there is a workgroup for all rows, and nothing is kept in the caches.
-template <typename T, int K, bool SUB, bool RES, bool RAGGED, bool ONCE>
+// registers; STREAM: nothing is kept in the caches.
+template <typename T, int K, bool SUB, bool RES, bool RAGGED, bool STREAM>
 __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int waves, int rows) {
   constexpr int VEC = Vec<T>::N;
   typedef typename Vec<T>::Type V;
@@ -280,15 +280,15 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int first = span_of<VEC>(k * at.threads + at.lane, n).first;
-      f.x[k] = load_vec<ONCE>((const T*)a.x + row * a.ldx + first);
-      if (RES) f.r[k] = load_vec<ONCE>((const T*)a.r + row * a.ldr + first);
+      f.x[k] = load_vec<STREAM>((const T*)a.x + row * a.ldx + first);
+      if (RES) f.r[k] = load_vec<STREAM>((const T*)a.r + row * a.ldr + first);
     }
   };
   const int64_t stride = (int64_t)gridDim.x * rows;
   int64_t begin = (int64_t)blockIdx.x * rows;   // the workgroup's first row of this turn
-  constexpr bool AHEAD = K <= 2 && !ONCE;
+  constexpr bool AHEAD = K <= 2;
   Row one, other;
-  if (AHEAD || ONCE) fetch(one, begin + at.group);
+  if (AHEAD) fetch(one, begin + at.group);
   float w[K][VEC], b[K][VEC];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
   // hold both.
   auto step = [&](Row& f, Row& next) -> bool {
     const int64_t row = begin + at.group;
-    const bool live = row < a.M, more = !ONCE && begin + stride < a.M;
-    if (!AHEAD && !ONCE) fetch(f, row);
+    const bool live = row < a.M, more = begin + stride < a.M;
+    if (!AHEAD) fetch(f, row);
     if (AHEAD && more) fetch(next, row + stride);
     float h[K][VEC], s[1] = {0.0f};
 #pragma unroll
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
       if (RES) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) f.x[k][e] = (T)((float)f.x[k][e] + (float)f.r[k][e]);
-        if (live && span.twice < VEC) store_vec<ONCE>((T*)a.h + row * a.N + span.first, f.x[k]);
+        if (live && span.twice < VEC) store_vec<STREAM>((T*)a.h + row * a.N + span.first, f.x[k]);
       }
       float t = 0.0f;
 #pragma unroll
@@ -349,8 +349,14 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
         if (span.twice == VEC) continue;
         V y;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) y[e] = (T)(h[k][e] * rstd * w[k][e] + b[k][e]);
-        store_vec<ONCE>((T*)a.y + row * a.N + span.first, y);
+        for (int e = 0; e < VEC; ++e) {
+          float f = h[k][e] * rstd * w[k][e] + b[k][e];
+          // (rounded to fp32 first with and without a residual: a mixed-precision multiply-add,
+          // which the compiler takes where it likes, would round once and give other bits)
+          asm volatile("" : "+v"(f));
+          y[e] = (T)f;
+        }
+        store_vec<STREAM>((T*)a.y + row * a.N + span.first, y);
       }
       if (at.lane == 0 && a.mean) {
         a.mean[row] = mean;
@@ -361,9 +367,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
     turn ^= 1;
     return more;
   };
-  if (ONCE) {
-    step(one, one);
-  } else if (AHEAD) {
+  if (AHEAD) {
     while (step(one, other) && step(other, one)) {
     }
   } else {
@@ -387,18 +391,19 @@ inline RowPlan plan_row(int64_t N, int vec, bool single) {
 }
 
 template <typename T, int K, bool SUB>
-int norm_rows_launch(const NormArgs& a, const RowPlan& plan, hipStream_t stream) {
+int norm_rows_launch(const NormArgs& a, const RowPlan& plan, hipStream_t queue) {
   const int rows = SUB ? 16 : plan.waves >= 4 ? 1 : 4 / plan.waves;
   const int threads = SUB ? 256 : plan.waves * rows * 64;
-  const bool once = a.r && 4 * a.M * a.N * (int64_t)sizeof(T) > kCached;
+  const bool stream = a.r && 4 * a.M * a.N * (int64_t)sizeof(T) > kCached;
   int64_t groups = ceil_div(a.M, rows);
-  const int64_t most = 256 * (2048 / threads) / 2;
-  if (!once && groups > most) groups = most;
+  const int64_t most = stream ? (groups + 1) / 2 : 256 * (2048 / threads) / 2;
+  if (groups > most) groups = most;
+  if (groups > kMostBlocks) groups = kMostBlocks;
   const bool ragged = a.N % Vec<T>::N != 0;
-#define AXN_NORM(RES, RAGGED, ONCE)                                                                              \
-  if ((a.r != nullptr) == RES && ragged == RAGGED && once == ONCE)                                               \
-  hipLaunchKernelGGL((norm_rows_kernel<T, K, SUB, RES, RAGGED, ONCE>), dim3((unsigned)groups), dim3(threads), 0, \
-                     stream, a, plan.waves, rows)
+#define AXN_NORM(RES, RAGGED, STREAM)                                                                              \
+  if ((a.r != nullptr) == RES && ragged == RAGGED && stream == STREAM)                                             \
+  hipLaunchKernelGGL((norm_rows_kernel<T, K, SUB, RES, RAGGED, STREAM>), dim3((unsigned)groups), dim3(threads), 0, \
+                     queue, a, plan.waves, rows)
   AXN_NORM(false, false, false);
   AXN_NORM(false, true, false);
   AXN_NORM(true, false, false);

@@ -432,6 +432,22 @@ def test_other_stream():
     check_backward(grads, dy, got[1], w, got[2], got[3], ds, torch.float16)
 
 
+@pytest.mark.parametrize("N", [64, 1024, 1027, 4160, 20000])
+def test_sums_larger_than_the_cache(N):
+    """With a residual, from 256 MB on: rows from all over the matrix, the last ones among them."""
+    from axonn_amd import ops
+
+    M = (300 << 20) // (8 * N) + 5
+    for params in ("same", "fp32"):
+        x, r, w, b, _, _ = make(M, N, torch.float16, params, seed=N, residual=True)
+        y, h, mean, rstd = ops.layer_norm_fwd(x, w, b, residual=r)
+        assert torch.equal(h, x + r)
+        rows = torch.cat([torch.arange(0, M, max(1, M // 50)), torch.arange(M - 5, M)]).cuda()
+        check_forward(y[rows], mean[rows], rstd[rows], h[rows], w, b, torch.float16)
+        z, _, _, _ = ops.layer_norm_fwd(h, w, b)      # without: the other kernel, of the same sums
+        assert torch.equal(z, y)
+
+
 def test_rows_beyond_32_bits():
     """The last rows of a matrix of more than 2^31 elements, and of one whose stride takes them there."""
     from axonn_amd import ops
