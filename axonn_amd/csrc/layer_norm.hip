@@ -30,7 +30,12 @@ __device__ __forceinline__ float param_at(const void* p, int wide, int64_t i) {
 }
 
 constexpr int ROW_THREADS = 256;
-constexpr int64_t kCached = 256 << 20;   // bytes that the memory-side cache holds
+constexpr int64_t kL2 = 32 << 20;        // bytes that the eight L2s hold
+// Bytes that the memory-side cache holds.  A forward with a residual that moves more keeps nothing in the
+// caches, in two turns a workgroup: 16384 x 8192 bf16 203 -> 180 us, with the product that reads it 368 ->
+// 374 (8192 x 8192 215 -> 206, 32768 x 8192 753 -> 739).  Without a residual there is nothing in it (98 us
+// -> 105, 279 -> 299).
+constexpr int64_t kCached = 256 << 20;
 constexpr int MOST_PARTS = 256;   // parts of the rows whose column sums meet in a second launch
 
 template <int THREADS>
@@ -53,7 +58,7 @@ struct NormArgs {
   float *mean, *rstd;
   int64_t M, N, ldx, ldr;
   float eps;
-  int wide;
+  int wide, through;
 };
 
 // Rows of any length, element by element, one workgroup to a row.
@@ -179,6 +184,21 @@ __device__ __forceinline__ void store_vec(T* p, typename Vec<T>::Type v) {
     __builtin_nontemporal_store(v, (typename Vec<T>::Type*)p);
   else
     *(typename Vec<T>::Type*)p = v;
+}
+// A vector of the forward's results.  Those of a call that the L2s can hold (`through`) are written
+// through them, or they are all written back when the kernel ends: 1024 x 4096 bf16 5.6 -> 4.8 us, with
+// the product that reads it 20.7 -> 19.8; 3001 x 1025 fp32 7.1 -> 5.8.  From 64 MB on there is nothing in
+// it (8192 x 8192 and its product 153 -> 164), and in the backward, with its second launch, little
+// (1000 x 4096 15.3 -> 14.9, 16384 x 5120 99 -> 100).
+// Results that bypass the caches take another 2 to 20 % less here and cost their reader more than that
+// (4096 x 4096 and its product 46 -> 54 us, 8192 x 8192 154 -> 169): not done (see kCached for the exception).
+template <bool NT, typename T>
+__device__ __forceinline__ void store_result(T* p, typename Vec<T>::Type v, int through) {
+  if (NT || !through) {
+    store_vec<NT>(p, v);
+  } else {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
+  }
 }
 // VEC parameters from element i on, as floats.
 template <typename T>
@@ -316,7 +336,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
       if (RES) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) f.x[k][e] = (T)((float)f.x[k][e] + (float)f.r[k][e]);
-        if (live && span.twice < VEC) store_vec<STREAM>((T*)a.h + row * a.N + span.first, f.x[k]);
+        if (live && span.twice < VEC) store_result<STREAM>((T*)a.h + row * a.N + span.first, f.x[k], a.through);
       }
       float t = 0.0f;
 #pragma unroll
@@ -356,7 +376,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
           asm volatile("" : "+v"(f));
           y[e] = (T)f;
         }
-        store_vec<STREAM>((T*)a.y + row * a.N + span.first, y);
+        store_result<STREAM>((T*)a.y + row * a.N + span.first, y, a.through);
       }
       if (at.lane == 0 && a.mean) {
         a.mean[row] = mean;
@@ -688,7 +708,8 @@ size_t layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
 int launch_layer_norm_fwd(const void* x, const void* r, const void* w, const void* b, void* y, void* h, float* mean,
                           float* rstd, int dtype, bool wide, int64_t M, int64_t N, int64_t ldx, int64_t ldr, float eps,
                           hipStream_t stream) {
-  const NormArgs a = {x, r, w, b, y, h, mean, rstd, M, N, ldx, ldr, eps, wide};
+  const NormArgs a = {x, r, w, b, y, h, mean, rstd, M, N, ldx, ldr, eps, wide,
+                      M * N * (dtype == AXN_F32 ? 4 : 2) <= kL2};
   switch (dtype) {
     case AXN_BF16: return norm_launch<AXN_BF16>(a, stream);
     case AXN_F16: return norm_launch<AXN_F16>(a, stream);
