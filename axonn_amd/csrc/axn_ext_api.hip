@@ -121,7 +121,7 @@ int axn_layer_norm_bwd(const void* dy, const void* h, const void* weight, const 
     CHECK(check_param(name, "mean", mean, 4));
     CHECK(check_param(name, "rstd", rstd, 4));
     CHECK(check_param(name, "dx", dx, es));
-    if (dweight || dbias) {
+    if ((dweight || dbias) && layer_norm_bwd_workspace_bytes(M, N) > 0) {
       REQUIRE(workspace != nullptr && workspace_bytes >= layer_norm_bwd_workspace_bytes(M, N), AXN_EINVAL,
               "%s: workspace too small (%zu bytes given, %zu needed)", name, workspace_bytes,
               layer_norm_bwd_workspace_bytes(M, N));

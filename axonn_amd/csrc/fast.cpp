@@ -485,7 +485,9 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
   const bool eight = args[8] != Py_None;
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
-  const c10::DeviceIndex device = c10::hip::current_device();
+  PyObject* first = PyList_GET_ITEM(args[0], 0);
+  if (!THPVariable_CheckExact(first)) Py_RETURN_NONE;
+  const c10::DeviceIndex device = current_device_for(THPVariable_Unpack(first));   // (no device is asked for a CPU tensor)
   std::vector<int64_t> sizes;
   sizes.reserve(n);
   TensorList g, p, m, v, low;

@@ -161,6 +161,9 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_dparam_sum_kernel(const Norm
 }
 
 // ---------------------------------------------------------- vector kernels --
+// Both passes are bound by memory: a row's elements are read once and written once.  A copy on the
+// same GPU moves 6.8 TB/s; the forward moves 5.1 to 5.9 TB/s of bf16 from 20 MB on, the backward 4 to
+// 5.5 (see there).
 // A row lies in the registers of 16 lanes or of several whole waves, K vectors of 16 bytes in a
 // lane, and is read once.
 // Vector v of a row holds its elements from v VEC on, but the last one ends with the row and
@@ -282,6 +285,8 @@ __device__ __forceinline__ void row_sums(float (&x)[COUNT], const RowOf<SUB>& at
   }
 }
 
+// The next row is on its way while one is summed.  Twice as many workgroups as are resident half full
+// measured 5 to 8 % slower, half as many up to 13 % (most in norm_rows_launch).
 // RES: a residual is added.  RAGGED: N is no multiple of a vector.  A workgroup takes `rows` rows at
 // a time and goes on to those gridDim.x workgroups further, the parameters of its columns in
 // registers; STREAM: nothing is kept in the caches.
@@ -397,7 +402,9 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormArgs a, int w
 }
 
 // Waves and vectors of a lane for rows of N elements, and whether 16 lanes do.  `single`: one vector
-// to a lane as long as 16 waves hold the row.
+// to a lane as long as 16 waves hold the row, which the backward takes: its sums of columns then take
+// half the registers (bf16 4096 x 4096 28.9 -> 27.0 us, 16384 x 5120 104 -> 99.5).  The forward, which
+// has none, is faster with two (4096 x 4096 13.1 us, 15.7 with one; 8192 x 5120 33, 45).
 struct RowPlan {
   int k, waves;
   bool sub;
@@ -443,7 +450,12 @@ int norm_rows(const NormArgs& a, hipStream_t stream) {
   return norm_rows_launch<T, 4, false>(a, plan, stream);
 }
 
-// Backward: rows as above, several at a time in a workgroup, which goes on to the rows `parts`
+// Backward.  Its time is 11 us and the bytes at 5.7 TB/s: 3 us to launch and to the first rows, 3 for
+// the workgroups' sums (8 MB of them for 4096 columns, written at the end), 4 to 5 for the second launch
+// that adds them up.  256 workgroups of up to 16 waves, one to a CU, are a compromise: 512 of half the
+// size, two to a CU, are 5 % faster up to their sums and 5 to 15 % slower with twice as many of those.
+// 4096 x 4096 bf16 with dsum 32.7 us (4.1 TB/s), 16384 x 5120 98 us (5.1), 32768 x 4096 147 us (5.5).
+// Rows as above, several at a time in a workgroup, which goes on to the rows `parts`
 // workgroups further until there are none.  Its threads keep the sums of dy xhat and dy of their
 // columns in registers; at the end the workgroup's rows are joined in LDS and its sums go to
 // `partial`.  RAGGED: N is no multiple of a vector.  SUM: dsum is given.
@@ -587,7 +599,8 @@ __global__ void __launch_bounds__(1024) norm_grad_rows_kernel(const NormGradArgs
 }
 
 // The workgroups' sums added up: 32 of the 2 N columns to a workgroup, 16 threads to a column,
-// each taking every 16th part.
+// each taking every 16th part: all loads of the launch are on their way at once, lines of 128 bytes
+// each.  8 MB in 4 us; 16 columns to a workgroup 5.5, four columns to a thread 6.
 constexpr int JOIN_COLUMNS = 32, JOIN_SLICES = 16;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_COLUMNS* JOIN_SLICES) norm_grad_join_kernel(const NormGradArgs a) {
@@ -661,6 +674,82 @@ int norm_grad_rows(const NormGradArgs& a, hipStream_t stream) {
   return norm_grad_rows_launch<T, 4, false>(a, plan, stream);
 }
 
+// Backward of few rows in one launch and without a workspace: the sums over rows need nothing of the
+// sums along them.  The first a.M workgroups take a row each, in vectors and from the caches the
+// second time, the others FEW_COLUMNS columns each and all rows, FEW_SLICES threads to a column.
+constexpr int FEW_COLUMNS = 32, FEW_SLICES = 8;
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS) norm_grad_few_kernel(const NormGradArgs a) {
+  constexpr int VEC = Vec<T>::N;
+  typedef typename Vec<T>::Type V;
+  __shared__ float shared[2][FEW_SLICES][FEW_COLUMNS];
+  const int n = (int)a.N, rows = a.dx ? (int)a.M : 0, t = threadIdx.x;
+  if ((int)blockIdx.x < rows) {
+    const int64_t row = blockIdx.x;
+    const T *dy = (const T*)a.dy + row * a.lddy, *h = (const T*)a.h + row * a.ldh;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    const int vectors = (n + VEC - 1) / VEC;
+    float s1 = 0.0f, s2 = 0.0f, w[VEC];
+    for (int v = t; v < vectors; v += ROW_THREADS) {
+      const Span span = span_of<VEC>(v, n);
+      const V d = load_vec(dy + span.first), x = load_vec(h + span.first);
+      if (a.w) load_params<T>(a.w, a.wide, span.first, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float g = e < span.twice ? 0.0f : (float)d[e] * (a.w ? w[e] : 1.0f);
+        s1 += g;
+        s2 += g * ((float)x[e] - mean);
+      }
+    }
+    float* meet = &shared[0][0][0];
+    const float shift = block_sum<ROW_THREADS>(s1, meet) / (float)n * rstd;
+    const float slope = block_sum<ROW_THREADS>(s2, meet) / (float)n * rstd * rstd;
+    for (int v = t; v < vectors; v += ROW_THREADS) {
+      const Span span = span_of<VEC>(v, n);
+      const V d = load_vec(dy + span.first), x = load_vec(h + span.first);
+      V extra, out;
+      if (a.dsum) extra = load_vec((const T*)a.dsum + row * a.ldsum + span.first);
+      if (a.w) load_params<T>(a.w, a.wide, span.first, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float g = (float)d[e] * (a.w ? w[e] : 1.0f) * rstd - shift;
+        g -= ((float)x[e] - mean) * rstd * slope;
+        if (a.dsum) g += (float)extra[e];
+        out[e] = (T)g;
+      }
+      store_vec((T*)a.dx + row * a.N + span.first, out);
+    }
+    return;
+  }
+  const int lane = t % FEW_COLUMNS, slice = t / FEW_COLUMNS;
+  const int64_t col = (int64_t)(blockIdx.x - rows) * FEW_COLUMNS + lane;
+  float dw = 0.0f, db = 0.0f;
+  if (col < n) {
+#pragma unroll 8
+    for (int row = slice; row < (int)a.M; row += FEW_SLICES) {
+      const float d = (float)((const T*)a.dy)[row * a.lddy + col];
+      dw += d * (((float)((const T*)a.h)[row * a.ldh + col] - a.mean[row]) * a.rstd[row]);
+      db += d;
+    }
+  }
+  shared[0][slice][lane] = dw;
+  shared[1][slice][lane] = db;
+  __syncthreads();
+  if (slice > 1 || col >= n) return;
+  void* out = slice == 0 ? a.dw : a.db;
+  if (!out) return;
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < FEW_SLICES; ++i) s += shared[slice][i][lane];
+  if (a.wide) ((float*)out)[col] = s; else ((T*)out)[col] = (T)s;
+}
+
+// Up to 512 rows (from 16 elements on, so that a vector fits).  us, two launches / this one: 64 x 1024
+// fp32 7.4 / 5.0, 400 x 1024 10.1 / 6.0, 800 x 1024 10.6 / 11.3; 256 x 4096 bf16 10.6 / 5.5, 800 x 4096
+// 14.7 / 12.5, 1100 x 4096 16.4 / 15.8; 128 x 12288 16.4 / 10.2, 600 x 12288 21.4 / 19.7, 800 x 12288 23.9 /
+// 27.0; 400 x 8192 fp32 14.7 / 13.8, 600 x 8192 17.1 / 20.3.
+inline bool few_rows(int64_t M, int64_t N) { return M >= 1 && M <= 512 && N >= 16; }
+
 template <int DT>
 int norm_launch(const NormArgs& a, hipStream_t stream) {
   typedef typename Elem<DT>::type T;
@@ -673,6 +762,12 @@ int norm_launch(const NormArgs& a, hipStream_t stream) {
 template <int DT>
 int norm_grad_launch(const NormGradArgs& a, hipStream_t stream) {
   typedef typename Elem<DT>::type T;
+  if (few_rows(a.M, a.N)) {
+    const int64_t groups = (a.dx ? a.M : 0) + (a.dw || a.db ? ceil_div(a.N, FEW_COLUMNS) : 0);
+    hipLaunchKernelGGL(norm_grad_few_kernel<T>, dim3((unsigned)groups), dim3(ROW_THREADS), 0, stream, a);
+    AXN_HIP_TRY(hipGetLastError());
+    return AXN_OK;
+  }
   if (a.M > 0 && a.N >= Vec<T>::N && a.N <= 4096 * Vec<T>::N) return norm_grad_rows<T>(a, stream);
   if (a.dx) {
     hipLaunchKernelGGL(norm_dx_any_kernel<T>, grid_of(a.M), dim3(ROW_THREADS), 0, stream, a);
@@ -701,7 +796,7 @@ int norm_grad_parts(int64_t M) {
 }  // namespace
 
 size_t layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
-  if (M < 1 || N < 1) return 0;
+  if (M < 1 || N < 1 || few_rows(M, N)) return 0;
   return (size_t)(M < MOST_PARTS ? M : MOST_PARTS) * 2 * (size_t)N * sizeof(float);
 }
 

@@ -48,7 +48,8 @@ AXN_API int axn_layer_norm_fwd(const void* x, const void* residual, const void* 
  *   have param_dtype, are summed in fp32 in a fixed order (equal calls give equal
  *   bits) and rounded once.
  *   workspace: axn_layer_norm_bwd_workspace_bytes(M, N) bytes, 16-byte aligned,
- *   used by this call alone until it has finished; needed for dweight and dbias.
+ *   used by this call alone until it has finished; needed for dweight and dbias
+ *   unless it is of 0 bytes.
  * M = 0 writes zeros to dweight and dbias. */
 AXN_API size_t axn_layer_norm_bwd_workspace_bytes(int64_t M, int64_t N);
 AXN_API int axn_layer_norm_bwd(const void* dy, const void* h, const void* weight, const float* mean,

@@ -98,7 +98,8 @@ def check_backward(got, dy, h, w, mean, rstd, ds, dtype):
 
 SIZES = [(1, 1), (3, 2), (2, 7), (5, 8), (7, 63), (16, 64), (9, 100), (4, 129), (33, 256), (3, 1000), (17, 1025),
          (64, 1024), (5, 2049), (3, 4096), (2, 4099), (3, 5120), (2, 8192), (3, 8200), (1, 16384), (2, 16387), (2, 32768),
-         (2, 32776), (2, 40001), (300, 520), (1030, 96), (4097, 24)]
+         (2, 32776), (2, 40001), (300, 520), (1030, 96), (4097, 24), (512, 1000), (513, 1000), (513, 40001), (600, 15), (520, 8),
+         (700, 9000), (530, 16388), (515, 32768)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -129,12 +130,12 @@ def test_rows_of_other_strides_and_alignments(dtype):
     """Views of wider buffers, at odd places, with odd strides; what is around them is left alone."""
     from axonn_amd import ops
 
-    for N in (64, 100, 1024, 1027, 4096, 8200):
+    for M, N in ((5, 64), (5, 100), (5, 1024), (5, 1027), (5, 4096), (5, 8200), (600, 64), (600, 1027), (515, 8200)):
         for skip, ld in ((1, N + 3), (8, N + 16), (5, N + 8)):
-            x, r, w, b, dy, ds = make(5, N, dtype, "same", seed=N, residual=True)
+            x, r, w, b, dy, ds = make(M, N, dtype, "same", seed=N, residual=True)
             wide = []
             for t in (x, r, dy, ds):
-                big = torch.full((5, ld + skip), 777.0, device="cuda").to(dtype)
+                big = torch.full((M, ld + skip), 777.0, device="cuda").to(dtype)
                 big[:, skip:skip + N] = t
                 wide.append(big[:, skip:skip + N])
             apart = torch.cat([torch.zeros(1, device="cuda", dtype=dtype), w])[1:]   # (a parameter at an odd place too)
@@ -153,35 +154,36 @@ def test_rows_of_other_strides_and_alignments(dtype):
     check_forward(*[ops.layer_norm_fwd(x)[i] for i in (0, 2, 3)], x, None, None, dtype)
 
 
-@pytest.mark.parametrize("N", [63, 64, 1024, 4096, 8200, 40001])
-def test_outputs_end_where_their_rows_do(N):
+@pytest.mark.parametrize("M,N", [(3, 63), (3, 64), (3, 1024), (3, 4096), (3, 8200), (3, 40001), (517, 63), (517, 64), (517, 1030),
+                                 (517, 8200), (517, 40001)])
+def test_outputs_end_where_their_rows_do(M, N):
     """Through the C ABI into buffers with something behind them (and in front), M rows of them."""
     from axonn_amd import _native as nv
 
     for dtype in DTYPES:
-        x, r, w, b, dy, ds = make(3, N, dtype, "fp32", seed=N, residual=True)
-        guard, n = 64, 3 * N
+        x, r, w, b, dy, ds = make(M, N, dtype, "fp32", seed=N, residual=True)
+        guard, n = 64, M * N
         buf = {k: torch.full((n + 2 * guard,), 55.0, device="cuda").to(dtype) for k in ("y", "h", "dx")}
         par = {k: torch.full((N + 2 * guard,), 55.0, device="cuda") for k in ("dw", "db")}
-        st = {k: torch.full((3 + 2 * guard,), 55.0, device="cuda") for k in ("mean", "rstd")}
+        st = {k: torch.full((M + 2 * guard,), 55.0, device="cuda") for k in ("mean", "rstd")}
         at = lambda t: t.data_ptr() + guard * t.element_size()  # noqa: E731
         lib = nv.load()
         code = nv.dtype_code(dtype)
-        nbytes = lib.axn_layer_norm_bwd_workspace_bytes(3, N)
+        nbytes = lib.axn_layer_norm_bwd_workspace_bytes(M, N)
         ws = torch.full((nbytes + 256,), 77, dtype=torch.uint8, device="cuda")
         nv.check(lib.axn_layer_norm_fwd(x.data_ptr(), r.data_ptr(), w.data_ptr(), b.data_ptr(), at(buf["y"]), at(buf["h"]),
-                                        at(st["mean"]), at(st["rstd"]), code, nv.F32, 3, N, N, N, EPS, nv.current_stream()))
+                                        at(st["mean"]), at(st["rstd"]), code, nv.F32, M, N, N, N, EPS, nv.current_stream()))
         nv.check(lib.axn_layer_norm_bwd(dy.data_ptr(), at(buf["h"]), w.data_ptr(), at(st["mean"]), at(st["rstd"]),
-                                        ds.data_ptr(), at(buf["dx"]), at(par["dw"]), at(par["db"]), code, nv.F32, 3, N, N, N,
+                                        ds.data_ptr(), at(buf["dx"]), at(par["dw"]), at(par["db"]), code, nv.F32, M, N, N, N,
                                         N, ws.data_ptr(), nbytes, nv.current_stream()))
         torch.cuda.synchronize()
         for t in (*buf.values(), *par.values(), *st.values()):
             assert (t[:guard] == 55).all() and (t[-guard:] == 55).all()
         assert (ws[nbytes:] == 77).all()
-        h = buf["h"][guard:guard + n].view(3, N)
-        mean, rstd = (st[k][guard:guard + 3] for k in ("mean", "rstd"))
-        check_forward(buf["y"][guard:guard + n].view(3, N), mean, rstd, h, w, b, dtype)
-        check_backward((buf["dx"][guard:guard + n].view(3, N), par["dw"][guard:guard + N], par["db"][guard:guard + N]), dy, h,
+        h = buf["h"][guard:guard + n].view(M, N)
+        mean, rstd = (st[k][guard:guard + M] for k in ("mean", "rstd"))
+        check_forward(buf["y"][guard:guard + n].view(M, N), mean, rstd, h, w, b, dtype)
+        check_backward((buf["dx"][guard:guard + n].view(M, N), par["dw"][guard:guard + N], par["db"][guard:guard + N]), dy, h,
                        w, mean, rstd, ds, dtype)
 
 
@@ -245,8 +247,8 @@ def test_no_rows():
 def test_gradients_one_by_one(want):
     from axonn_amd import ops
 
-    for N in (72, 1001, 4096, 40000):
-        x, _, w, _, dy, _ = make(37, N, torch.bfloat16)
+    for M, N in ((37, 72), (37, 1001), (37, 4096), (37, 40000), (600, 72), (600, 1001), (530, 4096), (515, 40000)):
+        x, _, w, _, dy, _ = make(M, N, torch.bfloat16)
         _, _, mean, rstd = ops.layer_norm_fwd(x, w)
         every = ops.layer_norm_bwd(dy, x, w, mean, rstd)
         some = ops.layer_norm_bwd(dy, x, w, mean, rstd, None, *map(bool, want))
@@ -385,11 +387,12 @@ def test_gradients_against_differences():
             assert abs((f64(grad) * u).sum() - want) < (chain(N) + 64) * U * terms + 1e-7 * terms
 
 
-def test_replayed_norm_equals_the_eager_one():
+@pytest.mark.parametrize("rows", [200, 2000])
+def test_replayed_norm_equals_the_eager_one(rows):
     """Forward and backward captured once, replayed with other inputs between eager calls of the same sizes."""
     from axonn_amd import ops
 
-    x, r, w, b, dy, ds = make(200, 1000, torch.bfloat16, "fp32", residual=True)
+    x, r, w, b, dy, ds = make(rows, 1000, torch.bfloat16, "fp32", residual=True)
 
     def both():
         y, h, mean, rstd = ops.layer_norm_fwd(x, w, b, residual=r)
