@@ -12,8 +12,13 @@ The package keeps the reference's Python surface for the one path it covers
     axonn_amd.checkpoint.save / load               (axonn/checkpoint.py)
     axonn_amd.models.transformers.parallelize      (axonn/models/transformers)
 
+beside it
+
+    axonn_amd.intra_layer.LayerNorm                torch.nn.LayerNorm, with the residual add in front
+    axonn_amd.optim.AdamW                          decoupled weight decay, moments in 32 or in 8 bits
+
 and runs all of its arithmetic in hand-written gfx950 kernels behind the C ABI
-of libaxn_gfx950.so (include/axn.h).  There is no CPU or library fallback.
+of libaxn_gfx950.so (include/axn.h, include/axn_ext.h).  There is no CPU or library fallback.
 """
 
 from . import axonn  # noqa: F401

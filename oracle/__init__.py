@@ -15,6 +15,12 @@ torch) computes on the per-GPU hot path at a 1 x 1 x 1 grid:
                   reference's calls reduce to on one rank); used for timing the
                   CPU baseline and as a second, independent checker
 
+and, for operators that the reference leaves to torch,
+
+  oracle.layer_norm  layer norm and its gradients from the formulas, in 64 bits
+  oracle.adamw       the AdamW step in 64 bits; the 8-bit moments' codes, exponents and
+                     random words as include/axn_ext.h defines them
+
 Only tests/, __graft_entry__.smoke() and bench.py's cpu_baseline leg may import
 this package, and only as the checker.  The shipped package (axonn_amd) never
 imports it and has no CPU fallback.
@@ -32,6 +38,11 @@ What pins the oracle (tests/test_oracle.py, tests/test_golden.py):
   - Adam: torch.optim.Adam(foreach=False) over several steps, the step-1 closed
     form, and a float64 evaluation of the same recurrences
   - loss-scale state machine: the transition table of inter_layer.py:281-301
+
+  - layer norm: torch's autograd in float64 and central differences; AdamW:
+    torch.optim.AdamW in float64; the 8-bit codes: round trips, octave borders, the
+    integer form of the definition, unbiased rounding over all words
+    (tests/test_adamw_oracle.py)
 
 Parity unpinned by any test of the reference itself: the optimizer step, the
 loss scaler and the overflow check (the reference has no test for them); they
