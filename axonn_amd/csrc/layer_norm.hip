@@ -744,11 +744,11 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_grad_few_kernel(const NormGr
   if (a.wide) ((float*)out)[col] = s; else ((T*)out)[col] = (T)s;
 }
 
-// Up to 512 rows (from 16 elements on, so that a vector fits).  us, two launches / this one: 64 x 1024
+// Up to 512 rows (of 16 elements on, so that a vector fits, and up to 2^20, so that the grid does).  us, two launches / this one: 64 x 1024
 // fp32 7.4 / 5.0, 400 x 1024 10.1 / 6.0, 800 x 1024 10.6 / 11.3; 256 x 4096 bf16 10.6 / 5.5, 800 x 4096
 // 14.7 / 12.5, 1100 x 4096 16.4 / 15.8; 128 x 12288 16.4 / 10.2, 600 x 12288 21.4 / 19.7, 800 x 12288 23.9 /
 // 27.0; 400 x 8192 fp32 14.7 / 13.8, 600 x 8192 17.1 / 20.3.
-inline bool few_rows(int64_t M, int64_t N) { return M >= 1 && M <= 512 && N >= 16; }
+inline bool few_rows(int64_t M, int64_t N) { return M >= 1 && M <= 512 && N >= 16 && N <= 1 << 20; }
 
 template <int DT>
 int norm_launch(const NormArgs& a, hipStream_t stream) {
@@ -787,17 +787,22 @@ int norm_grad_launch(const NormGradArgs& a, hipStream_t stream) {
   return AXN_OK;
 }
 
-// Into how many parts the rows are cut for the sums over them, element by element.
-int norm_grad_parts(int64_t M) {
-  const int64_t parts = ceil_div(M, 16);
-  return parts > MOST_PARTS ? MOST_PARTS : (int)parts;
+// Into how many parts the rows are cut for the sums over them, element by element: no more sums than
+// rows to add, and fewer for wide ones, whose columns fill the GPU by themselves.
+int norm_grad_parts(int64_t M, int64_t N) {
+  int64_t parts = ceil_div(M, 16);
+  if (parts > MOST_PARTS) parts = MOST_PARTS;
+  const int64_t most = (1 << 25) / N;
+  return (int)(parts <= most ? parts : most > 0 ? most : 1);
 }
 
 }  // namespace
 
 size_t layer_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
   if (M < 1 || N < 1 || few_rows(M, N)) return 0;
-  return (size_t)(M < MOST_PARTS ? M : MOST_PARTS) * 2 * (size_t)N * sizeof(float);
+  // (rows of up to 4096 vectors of 8: a sum of every workgroup, see norm_grad_rows_launch)
+  const int64_t parts = N > 32768 ? norm_grad_parts(M, N) : M < MOST_PARTS ? M : MOST_PARTS;
+  return (size_t)parts * 2 * (size_t)N * sizeof(float);
 }
 
 int launch_layer_norm_fwd(const void* x, const void* r, const void* w, const void* b, void* y, void* h, float* mean,
@@ -816,7 +821,7 @@ int launch_layer_norm_bwd(const void* dy, const void* h, const void* w, const fl
                           const void* dsum, void* dx, void* dw, void* db, int dtype, bool wide, int64_t M, int64_t N,
                           int64_t lddy, int64_t ldh, int64_t ldsum, void* ws, hipStream_t stream) {
   const NormGradArgs a = {dy, h, w, dsum, mean, rstd, dx, dw, db, (float*)ws, M, N, lddy, ldh, ldsum,
-                          norm_grad_parts(M), wide};
+                          M == 0 ? 0 : norm_grad_parts(M, N), wide};
   switch (dtype) {
     case AXN_BF16: return norm_grad_launch<AXN_BF16>(a, stream);
     case AXN_F16: return norm_grad_launch<AXN_F16>(a, stream);

@@ -99,7 +99,7 @@ def check_backward(got, dy, h, w, mean, rstd, ds, dtype):
 SIZES = [(1, 1), (3, 2), (2, 7), (5, 8), (7, 63), (16, 64), (9, 100), (4, 129), (33, 256), (3, 1000), (17, 1025),
          (64, 1024), (5, 2049), (3, 4096), (2, 4099), (3, 5120), (2, 8192), (3, 8200), (1, 16384), (2, 16387), (2, 32768),
          (2, 32776), (2, 40001), (300, 520), (1030, 96), (4097, 24), (512, 1000), (513, 1000), (513, 40001), (600, 15), (520, 8),
-         (700, 9000), (530, 16388), (515, 32768)]
+         (700, 9000), (530, 16388), (515, 32768), (3, (1 << 20) + 7)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
