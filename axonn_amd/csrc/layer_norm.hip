@@ -29,7 +29,6 @@ __device__ __forceinline__ float param_at(const void* p, int wide, int64_t i) {
   return wide ? ((const float*)p)[i] : (float)((const T*)p)[i];
 }
 
-constexpr int ROW_THREADS = 256;
 constexpr int64_t kL2 = 32 << 20;        // bytes that the eight L2s hold
 // Bytes that the memory-side cache holds.  A forward with a residual that moves more keeps nothing in the
 // caches, in two turns a workgroup: 16384 x 8192 bf16 203 -> 180 us, with the product that reads it 368 ->
@@ -37,20 +36,6 @@ constexpr int64_t kL2 = 32 << 20;        // bytes that the eight L2s hold
 // -> 105, 279 -> 299).
 constexpr int64_t kCached = 256 << 20;
 constexpr int MOST_PARTS = 256;   // parts of the rows whose column sums meet in a second launch
-
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float x, float* shared) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-  if (THREADS == 64) return x;
-  __syncthreads();   // (the sums of an earlier call have been read)
-  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = 0.0f;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) x += shared[w];
-  return x;
-}
 
 struct NormArgs {
   const void *x, *r, *w, *b;
@@ -61,38 +46,6 @@ struct NormArgs {
   int wide, through;
 };
 
-// Rows of any length, element by element, one workgroup to a row.
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) norm_any_kernel(const NormArgs a) {
-  __shared__ float shared[ROW_THREADS / 64];
-  const int64_t row = block_number();
-  if (row >= a.M) return;
-  const T* x = (const T*)a.x + row * a.ldx;
-  const T* r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
-  auto at = [&](int64_t i) -> float { return r ? (float)(T)((float)x[i] + (float)r[i]) : (float)x[i]; };
-  float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < a.N; i += ROW_THREADS) s += at(i);
-  const float mean = block_sum<ROW_THREADS>(s, shared) / (float)a.N;
-  s = 0.0f;
-  for (int64_t i = threadIdx.x; i < a.N; i += ROW_THREADS) {
-    const float d = at(i) - mean;
-    s += d * d;
-  }
-  const float rstd = 1.0f / sqrtf(block_sum<ROW_THREADS>(s, shared) / (float)a.N + a.eps);
-  for (int64_t i = threadIdx.x; i < a.N; i += ROW_THREADS) {
-    const float h = at(i);
-    float y = (h - mean) * rstd;
-    if (a.w) y *= param_at<T>(a.w, a.wide, i);
-    if (a.b) y += param_at<T>(a.b, a.wide, i);
-    ((T*)a.y)[row * a.N + i] = (T)y;
-    if (a.h) ((T*)a.h)[row * a.N + i] = (T)h;
-  }
-  if (threadIdx.x == 0 && a.mean) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
-  }
-}
-
 struct NormGradArgs {
   const void *dy, *h, *w, *dsum;
   const float *mean, *rstd;
@@ -101,64 +54,6 @@ struct NormGradArgs {
   int64_t M, N, lddy, ldh, ldsum;
   int parts, wide;
 };
-
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) norm_dx_any_kernel(const NormGradArgs a) {
-  __shared__ float shared[ROW_THREADS / 64];
-  const int64_t row = block_number();
-  if (row >= a.M) return;
-  const T* dy = (const T*)a.dy + row * a.lddy;
-  const T* h = (const T*)a.h + row * a.ldh;
-  const float mean = a.mean[row], rstd = a.rstd[row];
-  float s1 = 0.0f, s2 = 0.0f;
-  for (int64_t i = threadIdx.x; i < a.N; i += ROW_THREADS) {
-    const float g = (float)dy[i] * (a.w ? param_at<T>(a.w, a.wide, i) : 1.0f);
-    s1 += g;
-    s2 += g * (((float)h[i] - mean) * rstd);
-  }
-  s1 = block_sum<ROW_THREADS>(s1, shared) / (float)a.N;
-  s2 = block_sum<ROW_THREADS>(s2, shared) / (float)a.N;
-  for (int64_t i = threadIdx.x; i < a.N; i += ROW_THREADS) {
-    const float g = (float)dy[i] * (a.w ? param_at<T>(a.w, a.wide, i) : 1.0f);
-    float d = (g - s1 - ((float)h[i] - mean) * rstd * s2) * rstd;
-    if (a.dsum) d += (float)((const T*)a.dsum)[row * a.ldsum + i];
-    ((T*)a.dx)[row * a.N + i] = (T)d;
-  }
-}
-
-// Column sums of dy xhat and dy over the rows of one part: a thread to a column.
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) norm_dparam_any_kernel(const NormGradArgs a) {
-  const int64_t col = block_number() * ROW_THREADS + threadIdx.x;
-  if (col >= a.N) return;
-  const int part = blockIdx.z;
-  const int64_t first = a.M * part / a.parts, last = a.M * (part + 1) / a.parts;
-  float dw = 0.0f, db = 0.0f;
-  for (int64_t row = first; row < last; ++row) {
-    const float g = (float)((const T*)a.dy)[row * a.lddy + col];
-    dw += g * (((float)((const T*)a.h)[row * a.ldh + col] - a.mean[row]) * a.rstd[row]);
-    db += g;
-  }
-  a.partial[(int64_t)part * 2 * a.N + col] = dw;
-  a.partial[((int64_t)part * 2 + 1) * a.N + col] = db;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) norm_dparam_sum_kernel(const NormGradArgs a) {
-  const int64_t col = block_number() * ROW_THREADS + threadIdx.x;
-  if (col >= a.N) return;
-  float dw = 0.0f, db = 0.0f;
-  for (int part = 0; part < a.parts; ++part) {
-    dw += a.partial[(int64_t)part * 2 * a.N + col];
-    db += a.partial[((int64_t)part * 2 + 1) * a.N + col];
-  }
-  if (a.dw) {
-    if (a.wide) ((float*)a.dw)[col] = dw; else ((T*)a.dw)[col] = (T)dw;
-  }
-  if (a.db) {
-    if (a.wide) ((float*)a.db)[col] = db; else ((T*)a.db)[col] = (T)db;
-  }
-}
 
 // ---------------------------------------------------------- vector kernels --
 // Both passes are bound by memory: a row's elements are read once and written once.  A copy on the
@@ -231,6 +126,13 @@ template <int VEC>
 __device__ __forceinline__ Span span_of(int v, int n) {
   const int first = min(v * VEC, n - VEC);
   return {first, min(v * VEC - first, VEC)};
+}
+
+// The same for rows of up to 2^31 - 1 elements, a vector of the row itself.
+template <int VEC>
+__device__ __forceinline__ Span long_span(int v, int n) {
+  const int64_t end = ((int64_t)v + 1) * VEC;
+  return end <= n ? Span{v * VEC, 0} : Span{n - VEC, (int)(end - n)};
 }
 
 // The threads of a row: SUB: 16 lanes, else `waves` whole waves (16 at most).
@@ -625,6 +527,14 @@ __global__ void __launch_bounds__(JOIN_COLUMNS* JOIN_SLICES) norm_grad_join_kern
   if (a.wide) ((float*)out)[i] = total; else ((T*)out)[i] = (T)total;
 }
 
+template <typename T>
+int norm_grad_join(const NormGradArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL(norm_grad_join_kernel<T>, grid_of(ceil_div(2 * a.N, JOIN_COLUMNS)), dim3(JOIN_COLUMNS * JOIN_SLICES), 0,
+                     stream, a);
+  AXN_HIP_TRY(hipGetLastError());
+  return AXN_OK;
+}
+
 template <typename T, int K, bool SUB>
 int norm_grad_rows_launch(NormGradArgs a, const RowPlan& plan, hipStream_t stream) {
   const bool params = a.dw || a.db;
@@ -636,7 +546,6 @@ int norm_grad_rows_launch(NormGradArgs a, const RowPlan& plan, hipStream_t strea
   const int threads = SUB ? rows * 16 : plan.waves * rows * 64;
   const int64_t groups = ceil_div(a.M, rows);
   a.parts = groups < MOST_PARTS ? (int)groups : MOST_PARTS;
-  if (!params) a.partial = nullptr;
   const size_t lds = params && rows > 1 ? (size_t)threads * 2 * K * Vec<T>::N * sizeof(float) : 0;
   constexpr size_t MOST_LDS = 1024 * 2 * K * Vec<T>::N * sizeof(float);
 #define AXN_NORM_GRAD(RAGGED, SUM)                                                                                  \
@@ -656,12 +565,7 @@ int norm_grad_rows_launch(NormGradArgs a, const RowPlan& plan, hipStream_t strea
   if (!ragged && !a.dsum) AXN_NORM_GRAD(false, false);
 #undef AXN_NORM_GRAD
   AXN_HIP_TRY(hipGetLastError());
-  if (params) {
-    hipLaunchKernelGGL(norm_grad_join_kernel<T>, grid_of(ceil_div(2 * a.N, JOIN_COLUMNS)),
-                       dim3(JOIN_COLUMNS * JOIN_SLICES), 0, stream, a);
-    AXN_HIP_TRY(hipGetLastError());
-  }
-  return AXN_OK;
+  return params ? norm_grad_join<T>(a, stream) : AXN_OK;
 }
 
 template <typename T>
@@ -674,51 +578,138 @@ int norm_grad_rows(const NormGradArgs& a, hipStream_t stream) {
   return norm_grad_rows_launch<T, 4, false>(a, plan, stream);
 }
 
+// ------------------------------------------------------------- long rows ----
+// Rows beyond the registers of 16 waves: a workgroup of them to a row, which it reads once for each
+// sum and once more for the result, again from the caches.  Element by element with 256 threads
+// 4 x 40000 bf16 took 101 us, so 10; 1000 x 100000 654, so 117 (3.4 TB/s), its backward 890 and 286.
+constexpr int LONG_THREADS = 1024;
+
+// The sum over a workgroup, in all of its threads.
+template <int THREADS>
+__device__ __forceinline__ float block_sum(float x, float* shared) {
+  constexpr int WAVES = THREADS / 64;
+  x = wave64_sum(x);
+  __syncthreads();   // (the sums of an earlier call have been read)
+  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = 0.0f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) x += shared[w];
+  return x;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(LONG_THREADS) norm_long_kernel(const NormArgs a) {
+  constexpr int VEC = Vec<T>::N;
+  typedef typename Vec<T>::Type V;
+  __shared__ float shared[LONG_THREADS / 64];
+  const int64_t row = block_number();
+  if (row >= a.M) return;
+  const T *x = (const T*)a.x + row * a.ldx, *r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
+  const int n = (int)a.N, vectors = (n - 1) / VEC + 1;
+  auto at = [&](int first) -> V {
+    V v = load_vec(x + first);
+    if (r) {
+      const V o = load_vec(r + first);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = (T)((float)v[e] + (float)o[e]);
+    }
+    return v;
+  };
+  float s = 0.0f;
+#pragma unroll 4
+  for (int v = threadIdx.x; v < vectors; v += LONG_THREADS) {
+    const Span span = long_span<VEC>(v, n);
+    const V h = at(span.first);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s += e < span.twice ? 0.0f : (float)h[e];
+  }
+  const float mean = block_sum<LONG_THREADS>(s, shared) / (float)n;
+  s = 0.0f;
+#pragma unroll 4
+  for (int v = threadIdx.x; v < vectors; v += LONG_THREADS) {
+    const Span span = long_span<VEC>(v, n);
+    const V h = at(span.first);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = e < span.twice ? 0.0f : (float)h[e] - mean;
+      s += d * d;
+    }
+  }
+  const float rstd = 1.0f / sqrtf(block_sum<LONG_THREADS>(s, shared) / (float)n + a.eps);
+  for (int v = threadIdx.x; v < vectors; v += LONG_THREADS) {
+    const Span span = long_span<VEC>(v, n);
+    const V h = at(span.first);
+    float w[VEC], b[VEC];
+    if (a.w) load_params<T>(a.w, a.wide, span.first, w);
+    if (a.b) load_params<T>(a.b, a.wide, span.first, b);
+    V y;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float f = ((float)h[e] - mean) * rstd * (a.w ? w[e] : 1.0f) + (a.b ? b[e] : 0.0f);
+      asm volatile("" : "+v"(f));   // (see norm_rows_kernel)
+      y[e] = (T)f;
+    }
+    store_vec((T*)a.y + row * a.N + span.first, y);
+    if (r) store_vec((T*)a.h + row * a.N + span.first, h);
+  }
+  if (threadIdx.x == 0 && a.mean) {
+    a.mean[row] = mean;
+    a.rstd[row] = rstd;
+  }
+}
+
+// dx of one row by a workgroup of THREADS, in vectors and from the caches the second time.
+template <typename T, int THREADS>
+__device__ __forceinline__ void dx_of_row(const NormGradArgs& a, int64_t row, float* shared) {
+  constexpr int VEC = Vec<T>::N;
+  typedef typename Vec<T>::Type V;
+  const int n = (int)a.N, vectors = (n - 1) / VEC + 1;
+  const T *dy = (const T*)a.dy + row * a.lddy, *h = (const T*)a.h + row * a.ldh;
+  const float mean = a.mean[row], rstd = a.rstd[row];
+  float s1 = 0.0f, s2 = 0.0f, w[VEC];
+#pragma unroll 2
+  for (int v = threadIdx.x; v < vectors; v += THREADS) {
+    const Span span = long_span<VEC>(v, n);
+    const V d = load_vec(dy + span.first), x = load_vec(h + span.first);
+    if (a.w) load_params<T>(a.w, a.wide, span.first, w);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float g = e < span.twice ? 0.0f : (float)d[e] * (a.w ? w[e] : 1.0f);
+      s1 += g;
+      s2 += e < span.twice ? 0.0f : g * ((float)x[e] - mean);
+    }
+  }
+  const float shift = block_sum<THREADS>(s1, shared) / (float)n * rstd;
+  const float slope = block_sum<THREADS>(s2, shared) / (float)n * rstd * rstd;
+#pragma unroll 2
+  for (int v = threadIdx.x; v < vectors; v += THREADS) {
+    const Span span = long_span<VEC>(v, n);
+    const V d = load_vec(dy + span.first), x = load_vec(h + span.first);
+    V extra, out;
+    if (a.dsum) extra = load_vec((const T*)a.dsum + row * a.ldsum + span.first);
+    if (a.w) load_params<T>(a.w, a.wide, span.first, w);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float g = (float)d[e] * (a.w ? w[e] : 1.0f) * rstd - shift;
+      g -= ((float)x[e] - mean) * rstd * slope;
+      if (a.dsum) g += (float)extra[e];
+      out[e] = (T)g;
+    }
+    store_vec((T*)a.dx + row * a.N + span.first, out);
+  }
+}
+
 // Backward of few rows in one launch and without a workspace: the sums over rows need nothing of the
 // sums along them.  The first a.M workgroups take a row each, in vectors and from the caches the
 // second time, the others FEW_COLUMNS columns each and all rows, FEW_SLICES threads to a column.
-constexpr int FEW_COLUMNS = 32, FEW_SLICES = 8;
+constexpr int FEW_COLUMNS = 32, FEW_SLICES = 8, FEW_THREADS = FEW_COLUMNS * FEW_SLICES;
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) norm_grad_few_kernel(const NormGradArgs a) {
-  constexpr int VEC = Vec<T>::N;
-  typedef typename Vec<T>::Type V;
+__global__ void __launch_bounds__(FEW_THREADS) norm_grad_few_kernel(const NormGradArgs a) {
   __shared__ float shared[2][FEW_SLICES][FEW_COLUMNS];
   const int n = (int)a.N, rows = a.dx ? (int)a.M : 0, t = threadIdx.x;
   if ((int)blockIdx.x < rows) {
-    const int64_t row = blockIdx.x;
-    const T *dy = (const T*)a.dy + row * a.lddy, *h = (const T*)a.h + row * a.ldh;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    const int vectors = (n + VEC - 1) / VEC;
-    float s1 = 0.0f, s2 = 0.0f, w[VEC];
-    for (int v = t; v < vectors; v += ROW_THREADS) {
-      const Span span = span_of<VEC>(v, n);
-      const V d = load_vec(dy + span.first), x = load_vec(h + span.first);
-      if (a.w) load_params<T>(a.w, a.wide, span.first, w);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float g = e < span.twice ? 0.0f : (float)d[e] * (a.w ? w[e] : 1.0f);
-        s1 += g;
-        s2 += g * ((float)x[e] - mean);
-      }
-    }
-    float* meet = &shared[0][0][0];
-    const float shift = block_sum<ROW_THREADS>(s1, meet) / (float)n * rstd;
-    const float slope = block_sum<ROW_THREADS>(s2, meet) / (float)n * rstd * rstd;
-    for (int v = t; v < vectors; v += ROW_THREADS) {
-      const Span span = span_of<VEC>(v, n);
-      const V d = load_vec(dy + span.first), x = load_vec(h + span.first);
-      V extra, out;
-      if (a.dsum) extra = load_vec((const T*)a.dsum + row * a.ldsum + span.first);
-      if (a.w) load_params<T>(a.w, a.wide, span.first, w);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float g = (float)d[e] * (a.w ? w[e] : 1.0f) * rstd - shift;
-        g -= ((float)x[e] - mean) * rstd * slope;
-        if (a.dsum) g += (float)extra[e];
-        out[e] = (T)g;
-      }
-      store_vec((T*)a.dx + row * a.N + span.first, out);
-    }
+    dx_of_row<T, FEW_THREADS>(a, blockIdx.x, &shared[0][0][0]);
     return;
   }
   const int lane = t % FEW_COLUMNS, slice = t / FEW_COLUMNS;
@@ -744,56 +735,196 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_grad_few_kernel(const NormGr
   if (a.wide) ((float*)out)[col] = s; else ((T*)out)[col] = (T)s;
 }
 
-// Up to 512 rows (of 16 elements on, so that a vector fits, and up to 2^20, so that the grid does).  us, two launches / this one: 64 x 1024
-// fp32 7.4 / 5.0, 400 x 1024 10.1 / 6.0, 800 x 1024 10.6 / 11.3; 256 x 4096 bf16 10.6 / 5.5, 800 x 4096
+// Up to 512 rows (of 16 elements on, so that a vector fits, and up to 2^20, so that the grid does).  us, two
+// launches / this one: 64 x 1024 fp32 7.4 / 5.0, 400 x 1024 10.1 / 6.0, 800 x 1024 10.6 / 11.3; 256 x 4096 bf16 10.6 / 5.5, 800 x 4096
 // 14.7 / 12.5, 1100 x 4096 16.4 / 15.8; 128 x 12288 16.4 / 10.2, 600 x 12288 21.4 / 19.7, 800 x 12288 23.9 /
 // 27.0; 400 x 8192 fp32 14.7 / 13.8, 600 x 8192 17.1 / 20.3.
 inline bool few_rows(int64_t M, int64_t N) { return M >= 1 && M <= 512 && N >= 16 && N <= 1 << 20; }
 
-template <int DT>
-int norm_launch(const NormArgs& a, hipStream_t stream) {
-  typedef typename Elem<DT>::type T;
-  if (a.N >= Vec<T>::N && a.N <= 4096 * Vec<T>::N) return norm_rows<T>(a, stream);
-  hipLaunchKernelGGL(norm_any_kernel<T>, grid_of(a.M), dim3(ROW_THREADS), 0, stream, a);
-  AXN_HIP_TRY(hipGetLastError());
-  return AXN_OK;
+template <typename T>
+__global__ void __launch_bounds__(LONG_THREADS) norm_dx_long_kernel(const NormGradArgs a) {
+  __shared__ float shared[LONG_THREADS / 64];
+  const int64_t row = block_number();
+  if (row < a.M) dx_of_row<T, LONG_THREADS>(a, row, shared);
 }
 
-template <int DT>
-int norm_grad_launch(const NormGradArgs& a, hipStream_t stream) {
-  typedef typename Elem<DT>::type T;
-  if (few_rows(a.M, a.N)) {
-    const int64_t groups = (a.dx ? a.M : 0) + (a.dw || a.db ? ceil_div(a.N, FEW_COLUMNS) : 0);
-    hipLaunchKernelGGL(norm_grad_few_kernel<T>, dim3((unsigned)groups), dim3(ROW_THREADS), 0, stream, a);
-    AXN_HIP_TRY(hipGetLastError());
-    return AXN_OK;
-  }
-  if (a.M > 0 && a.N >= Vec<T>::N && a.N <= 4096 * Vec<T>::N) return norm_grad_rows<T>(a, stream);
-  if (a.dx) {
-    hipLaunchKernelGGL(norm_dx_any_kernel<T>, grid_of(a.M), dim3(ROW_THREADS), 0, stream, a);
-    AXN_HIP_TRY(hipGetLastError());
-  }
-  if (a.dw || a.db) {
-    dim3 grid = grid_of(ceil_div(a.N, ROW_THREADS));
-    if (a.parts > 0) {   // (no rows: sums of nothing)
-      dim3 all = grid;
-      all.z = a.parts;
-      hipLaunchKernelGGL(norm_dparam_any_kernel<T>, all, dim3(ROW_THREADS), 0, stream, a);
-      AXN_HIP_TRY(hipGetLastError());
+// Column sums over the rows of one part: a thread to the columns of a vector.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_dparam_long_kernel(const NormGradArgs a) {
+  constexpr int VEC = Vec<T>::N;
+  typedef typename Vec<T>::Type V;
+  const int n = (int)a.N, v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= (n - 1) / VEC + 1) return;
+  const int first_col = long_span<VEC>(v, n).first;   // (of columns that two have, both have the same sums)
+  const int part = blockIdx.z;
+  const int64_t first = a.M * part / a.parts, last = a.M * (part + 1) / a.parts;
+  float dw[VEC], db[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) dw[e] = db[e] = 0.0f;
+#pragma unroll 4
+  for (int64_t row = first; row < last; ++row) {
+    const V d = load_vec((const T*)a.dy + row * a.lddy + first_col), x = load_vec((const T*)a.h + row * a.ldh + first_col);
+    const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      dw[e] += (float)d[e] * (((float)x[e] - mean) * rstd);
+      db[e] += (float)d[e];
     }
-    hipLaunchKernelGGL(norm_dparam_sum_kernel<T>, grid, dim3(ROW_THREADS), 0, stream, a);
-    AXN_HIP_TRY(hipGetLastError());
   }
-  return AXN_OK;
+  float* sums = a.partial + (int64_t)part * 2 * n + first_col;
+#pragma unroll
+  for (int e = 0; e < VEC; e += 4) {
+    store_vec(sums + e, Vec<float>::Type{dw[e], dw[e + 1], dw[e + 2], dw[e + 3]});
+    store_vec(sums + n + e, Vec<float>::Type{db[e], db[e + 1], db[e + 2], db[e + 3]});
+  }
 }
 
-// Into how many parts the rows are cut for the sums over them, element by element: no more sums than
-// rows to add, and fewer for wide ones, whose columns fill the GPU by themselves.
+// ------------------------------------------------------ rows below a vector --
+// Rows of fewer elements than a vector has: a thread to a row.  1000000 x 4 bf16 forward 934 us with a
+// workgroup to a row, 10 so; backward 1184 and 27.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_tiny_kernel(const NormArgs a) {
+  constexpr int MOST = Vec<T>::N - 1;
+  const int n = (int)a.N;
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.M; row += (int64_t)gridDim.x * 256) {
+    float h[MOST], s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      h[i] = 0.0f;
+      if (i >= n) continue;
+      h[i] = (float)((const T*)a.x)[row * a.ldx + i];
+      if (a.r) {
+        const T sum = (T)(h[i] + (float)((const T*)a.r)[row * a.ldr + i]);
+        ((T*)a.h)[row * a.N + i] = sum;
+        h[i] = (float)sum;
+      }
+      s += h[i];
+    }
+    const float mean = s / (float)n;
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      h[i] -= mean;
+      s += i < n ? h[i] * h[i] : 0.0f;
+    }
+    const float rstd = 1.0f / sqrtf(s / (float)n + a.eps);
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      if (i >= n) continue;
+      float f = h[i] * rstd * (a.w ? param_at<T>(a.w, a.wide, i) : 1.0f) + (a.b ? param_at<T>(a.b, a.wide, i) : 0.0f);
+      asm volatile("" : "+v"(f));   // (see norm_rows_kernel)
+      ((T*)a.y)[row * a.N + i] = (T)f;
+    }
+    if (a.mean) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) norm_grad_tiny_kernel(const NormGradArgs a) {
+  constexpr int MOST = Vec<T>::N - 1;
+  __shared__ float shared[4];
+  const int n = (int)a.N;
+  float dw[MOST], db[MOST], w[MOST];
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    dw[i] = db[i] = 0.0f;
+    w[i] = i < n && a.w ? param_at<T>(a.w, a.wide, i) : 1.0f;
+  }
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.M; row += (int64_t)a.parts * 256) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float g[MOST], xhat[MOST], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      g[i] = xhat[i] = 0.0f;
+      if (i >= n) continue;
+      const float d = (float)((const T*)a.dy)[row * a.lddy + i];
+      xhat[i] = ((float)((const T*)a.h)[row * a.ldh + i] - mean) * rstd;
+      dw[i] += d * xhat[i];
+      db[i] += d;
+      g[i] = d * w[i];
+      s1 += g[i];
+      s2 += g[i] * xhat[i];
+    }
+    if (!a.dx) continue;
+    s1 /= (float)n;
+    s2 /= (float)n;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      if (i >= n) continue;
+      float d = (g[i] - s1 - xhat[i] * s2) * rstd;
+      if (a.dsum) d += (float)((const T*)a.dsum)[row * a.ldsum + i];
+      ((T*)a.dx)[row * a.N + i] = (T)d;
+    }
+  }
+  if (!a.partial) return;
+  float* sums = a.partial + (int64_t)blockIdx.x * 2 * n;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    if (i >= n) continue;   // (for all threads alike)
+    const float sw = block_sum<256>(dw[i], shared), sb = block_sum<256>(db[i], shared);
+    if (threadIdx.x == 0) {
+      sums[i] = sw;
+      sums[n + i] = sb;
+    }
+  }
+}
+
+// Into how many parts the rows are cut for the column sums of long ones: no more sums than rows to add,
+// and fewer for wide ones, whose columns fill the GPU by themselves.
 int norm_grad_parts(int64_t M, int64_t N) {
   int64_t parts = ceil_div(M, 16);
   if (parts > MOST_PARTS) parts = MOST_PARTS;
   const int64_t most = (1 << 25) / N;
   return (int)(parts <= most ? parts : most > 0 ? most : 1);
+}
+
+template <int DT>
+int norm_launch(const NormArgs& a, hipStream_t stream) {
+  typedef typename Elem<DT>::type T;
+  if (a.N >= Vec<T>::N && a.N <= 4096 * Vec<T>::N) return norm_rows<T>(a, stream);
+  if (a.N < Vec<T>::N) {
+    const int64_t groups = ceil_div(a.M, 256);
+    hipLaunchKernelGGL(norm_tiny_kernel<T>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(norm_long_kernel<T>, grid_of(a.M), dim3(LONG_THREADS), 0, stream, a);
+  }
+  AXN_HIP_TRY(hipGetLastError());
+  return AXN_OK;
+}
+
+template <int DT>
+int norm_grad_launch(NormGradArgs a, hipStream_t stream) {
+  typedef typename Elem<DT>::type T;
+  const bool params = a.dw || a.db;
+  if (a.M == 0) return norm_grad_join<T>(a, stream);   // (sums of nothing)
+  if (few_rows(a.M, a.N)) {
+    const int64_t groups = (a.dx ? a.M : 0) + (params ? ceil_div(a.N, FEW_COLUMNS) : 0);
+    hipLaunchKernelGGL(norm_grad_few_kernel<T>, dim3((unsigned)groups), dim3(FEW_THREADS), 0, stream, a);
+    AXN_HIP_TRY(hipGetLastError());
+    return AXN_OK;
+  }
+  if (!params) a.partial = nullptr;
+  if (a.N >= Vec<T>::N && a.N <= 4096 * Vec<T>::N) return norm_grad_rows<T>(a, stream);
+  if (a.N < Vec<T>::N) {
+    const int64_t groups = ceil_div(a.M, 256);
+    a.parts = groups < MOST_PARTS ? (int)groups : MOST_PARTS;
+    hipLaunchKernelGGL(norm_grad_tiny_kernel<T>, dim3(a.parts), dim3(256), 0, stream, a);
+    AXN_HIP_TRY(hipGetLastError());
+    return params ? norm_grad_join<T>(a, stream) : AXN_OK;
+  }
+  if (a.dx) {
+    hipLaunchKernelGGL(norm_dx_long_kernel<T>, grid_of(a.M), dim3(LONG_THREADS), 0, stream, a);
+    AXN_HIP_TRY(hipGetLastError());
+  }
+  if (!params) return AXN_OK;
+  a.parts = norm_grad_parts(a.M, a.N);
+  const dim3 grid((unsigned)ceil_div(ceil_div(a.N, Vec<T>::N), 256), 1, a.parts);
+  hipLaunchKernelGGL(norm_dparam_long_kernel<T>, grid, dim3(256), 0, stream, a);
+  AXN_HIP_TRY(hipGetLastError());
+  return norm_grad_join<T>(a, stream);
 }
 
 }  // namespace
@@ -821,7 +952,7 @@ int launch_layer_norm_bwd(const void* dy, const void* h, const void* w, const fl
                           const void* dsum, void* dx, void* dw, void* db, int dtype, bool wide, int64_t M, int64_t N,
                           int64_t lddy, int64_t ldh, int64_t ldsum, void* ws, hipStream_t stream) {
   const NormGradArgs a = {dy, h, w, dsum, mean, rstd, dx, dw, db, (float*)ws, M, N, lddy, ldh, ldsum,
-                          M == 0 ? 0 : norm_grad_parts(M, N), wide};
+                          0, wide};
   switch (dtype) {
     case AXN_BF16: return norm_grad_launch<AXN_BF16>(a, stream);
     case AXN_F16: return norm_grad_launch<AXN_F16>(a, stream);

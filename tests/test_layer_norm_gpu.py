@@ -99,7 +99,7 @@ def check_backward(got, dy, h, w, mean, rstd, ds, dtype):
 SIZES = [(1, 1), (3, 2), (2, 7), (5, 8), (7, 63), (16, 64), (9, 100), (4, 129), (33, 256), (3, 1000), (17, 1025),
          (64, 1024), (5, 2049), (3, 4096), (2, 4099), (3, 5120), (2, 8192), (3, 8200), (1, 16384), (2, 16387), (2, 32768),
          (2, 32776), (2, 40001), (300, 520), (1030, 96), (4097, 24), (512, 1000), (513, 1000), (513, 40001), (600, 15), (520, 8),
-         (700, 9000), (530, 16388), (515, 32768), (3, (1 << 20) + 7)]
+         (700, 9000), (530, 16388), (515, 32768), (3, (1 << 20) + 7), (2000, 7), (70000, 3), ((1 << 20) + 300, 2)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -130,7 +130,8 @@ def test_rows_of_other_strides_and_alignments(dtype):
     """Views of wider buffers, at odd places, with odd strides; what is around them is left alone."""
     from axonn_amd import ops
 
-    for M, N in ((5, 64), (5, 100), (5, 1024), (5, 1027), (5, 4096), (5, 8200), (600, 64), (600, 1027), (515, 8200)):
+    for M, N in ((5, 64), (5, 100), (5, 1024), (5, 1027), (5, 4096), (5, 8200), (600, 64), (600, 1027), (515, 8200), (600, 3),
+                 (5, 40001), (515, 33000)):
         for skip, ld in ((1, N + 3), (8, N + 16), (5, N + 8)):
             x, r, w, b, dy, ds = make(M, N, dtype, "same", seed=N, residual=True)
             wide = []
@@ -154,7 +155,7 @@ def test_rows_of_other_strides_and_alignments(dtype):
     check_forward(*[ops.layer_norm_fwd(x)[i] for i in (0, 2, 3)], x, None, None, dtype)
 
 
-@pytest.mark.parametrize("M,N", [(3, 63), (3, 64), (3, 1024), (3, 4096), (3, 8200), (3, 40001), (517, 63), (517, 64), (517, 1030),
+@pytest.mark.parametrize("M,N", [(3, 3), (600, 2), (520, 33001), (3, 63), (3, 64), (3, 1024), (3, 4096), (3, 8200), (3, 40001), (517, 63), (517, 64), (517, 1030),
                                  (517, 8200), (517, 40001)])
 def test_outputs_end_where_their_rows_do(M, N):
     """Through the C ABI into buffers with something behind them (and in front), M rows of them."""
@@ -204,7 +205,7 @@ def test_rows_far_from_zero_and_without_spread(N):
     assert torch.isnan(ops.layer_norm_fwd(x, eps=0.0)[0]).all()
 
 
-@pytest.mark.parametrize("N", [40, 1024, 8192, 40000])
+@pytest.mark.parametrize("N", [3, 40, 1024, 8192, 40000])
 def test_values_that_are_not_finite_stay_in_their_row(N):
     from axonn_amd import ops
 
