@@ -9,6 +9,7 @@ counterpart in the reference, whose models use torch's own.
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import ops
@@ -57,7 +58,8 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, residual=N
     rows, n = x.shape, math.prod(shape)
     as_rows = [t if t is None else t.reshape(-1, n) for t in (x, residual)]
     params = [p if p is None else p.reshape(-1) for p in (weight, bias)]
-    if torch.is_grad_enabled():
+    # (tangents need no gradients: the autograd function, which has no rule for them, refuses them)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         out = _LayerNorm.apply(*as_rows, *params, eps, True)
     else:
         y, h, _, _ = ops.layer_norm_fwd(as_rows[0], *params, eps, residual=as_rows[1], save=False)
