@@ -16,15 +16,14 @@ from .. import ops
 
 
 class _LayerNorm(torch.autograd.Function):
-    """(y, h) of rows x, h = x or round(x + residual).  `save`: whether a backward pass may follow."""
+    """(y, h) of rows x, h = x or round(x + residual)."""
 
     @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps, save):
-        y, h, mean, rstd = ops.layer_norm_fwd(x, weight, bias, eps, residual=residual, save=save)
-        if save:
-            ctx.set_materialize_grads(False)
-            ctx.save_for_backward(x if h is None else h, weight, mean, rstd)
-            ctx.param_dtype = None if bias is None else bias.dtype
+    def forward(ctx, x, residual, weight, bias, eps):
+        y, h, mean, rstd = ops.layer_norm_fwd(x, weight, bias, eps, residual=residual)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if h is None else h, weight, mean, rstd)
+        ctx.param_dtype = None if bias is None else bias.dtype
         return y if h is None else (y, h)
 
     @staticmethod
@@ -37,7 +36,7 @@ class _LayerNorm(torch.autograd.Function):
         else:
             dx, dweight, dbias = ops.layer_norm_bwd(dy, h, weight, mean, rstd, dsum, need_x or need_residual, need_weight,
                                                     need_bias, ctx.param_dtype)
-        return dx if need_x else None, dx if need_residual else None, dweight, dbias, None, None
+        return dx if need_x else None, dx if need_residual else None, dweight, dbias, None
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, residual=None):
@@ -58,9 +57,10 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, residual=N
     rows, n = x.shape, math.prod(shape)
     as_rows = [t if t is None else t.reshape(-1, n) for t in (x, residual)]
     params = [p if p is None else p.reshape(-1) for p in (weight, bias)]
-    # (tangents need no gradients: the autograd function, which has no rule for them, refuses them)
-    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
-        out = _LayerNorm.apply(*as_rows, *params, eps, True)
+    # (without gradients too the autograd function is what refuses a tangent, for which it has no rule, and what a trace
+    # records; a trace may run with gradients later, so that the function always keeps what they need)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0 or torch.jit.is_tracing():
+        out = _LayerNorm.apply(*as_rows, *params, eps)
     else:
         y, h, _, _ = ops.layer_norm_fwd(as_rows[0], *params, eps, residual=as_rows[1], save=False)
         out = y if h is None else (y, h)

@@ -51,3 +51,22 @@ def test_a_layer_without_gradients_keeps_no_statistics(launches):
     assert launches == [False, False]
     layer(x)
     assert launches[2:] == [True]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("gradients", [True, False])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_a_trace_computes_what_the_layer_does(launches, gradients, with_residual):
+    """The call itself is in the graph, whatever mode it is recorded in and run in, and not the memory it filled."""
+    layer = LayerNorm(8)
+    with torch.no_grad():
+        layer.weight.mul_(1.5)
+    operands = lambda: tuple(torch.randn(3, 8) for _ in range(1 + with_residual))  # noqa: E731
+    with torch.set_grad_enabled(gradients):
+        traced = torch.jit.trace(layer, operands(), check_trace=False)
+    for again in (False, True, False):
+        args = operands()
+        with torch.set_grad_enabled(again):
+            got, want = traced(*args), layer(*args)
+        for a, b in zip(*((got, want) if with_residual else ((got,), (want,)))):
+            assert torch.equal(a, b) and a.requires_grad == again
