@@ -451,12 +451,13 @@ PyObject* layer_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ---- AdamW ---------------------------------------------------------------------------------
-// The pointers of a list of dense tensors of one type on the current device, and their sizes into
-// `sizes` if that is empty; a size of its own for each is else in `expected`.
+// The pointers of a list of dense tensors of one type on the current device, and their sizes into `sizes` if that is
+// empty; else each has `per` elements for every `unit` of its size begun.  `written`: tensors that share their memory
+// until the first write are given their own.
 struct TensorList {
   std::vector<void*> at;
   at::ScalarType type = at::ScalarType::Undefined;
-  bool take(PyObject* list, Py_ssize_t n, c10::DeviceIndex device, std::vector<int64_t>* sizes, int64_t per, int64_t unit) {
+  bool take(PyObject* list, Py_ssize_t n, c10::DeviceIndex device, std::vector<int64_t>* sizes, int64_t per, int64_t unit, bool written) {
     if (!PyList_CheckExact(list) || PyList_GET_SIZE(list) != n) return false;
     const bool first = sizes->empty();
     at.reserve(n);
@@ -469,7 +470,7 @@ struct TensorList {
       if (t.scalar_type() != type) return false;
       if (first) sizes->push_back(t.numel());
       else if (t.numel() != ((*sizes)[i] + unit - 1) / unit * per) return false;
-      at.push_back(const_cast<void*>(t.const_data_ptr()));
+      at.push_back(written ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr()));
     }
     return true;
   }
@@ -492,10 +493,10 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   sizes.reserve(n);
   TensorList g, p, m, v, low;
   const bool copy = args[4] != Py_None;
-  if (!g.take(args[0], n, device, &sizes, 1, 1) || !p.take(args[1], n, device, &sizes, 1, 1) ||
-      !m.take(args[2], n, device, &sizes, eight ? 2 * AXN_ADAMW8_BLOCK : 1, eight ? AXN_ADAMW8_BLOCK : 1) ||
-      !v.take(args[3], n, device, &sizes, eight ? 2 : 1, eight ? AXN_ADAMW8_BLOCK : 1) ||
-      (copy && !low.take(args[4], n, device, &sizes, 1, 1)))
+  if (!g.take(args[0], n, device, &sizes, 1, 1, false) || !p.take(args[1], n, device, &sizes, 1, 1, true) ||
+      !m.take(args[2], n, device, &sizes, eight ? 2 * AXN_ADAMW8_BLOCK : 1, eight ? AXN_ADAMW8_BLOCK : 1, true) ||
+      !v.take(args[3], n, device, &sizes, eight ? 2 : 1, eight ? AXN_ADAMW8_BLOCK : 1, true) ||
+      (copy && !low.take(args[4], n, device, &sizes, 1, 1, true)))
     Py_RETURN_NONE;
   const at::ScalarType state = eight ? at::kByte : at::kFloat;
   if (!known(g.type) || p.type != at::kFloat || m.type != state || v.type != state || (copy && !is16(low.type))) Py_RETURN_NONE;
