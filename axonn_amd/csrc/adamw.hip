@@ -379,7 +379,7 @@ int launch_mt_adamw(const void* const* h_g, void* const* h_p, void* const* h_m, 
   s.hp = hp;
   s.inv_scale = inv_scale;
   const bool has_plow = h_plow != nullptr;
-  return for_each_group(sets, es, 5, h_sizes, n, ADAM_CHUNK, [&](const Group& gr) {
+  return for_each_group(sets, es, 5, h_sizes, n, ADAM_CHUNK, ADAM_THREADS, [&](const Group& gr) {
     switch (g_dtype) {
 #define AXN_ADAMW_CASE(GDT)                                                                    \
   return scan != nullptr ? adamw_launch<GDT, true>(gr, s, plow_dtype, has_plow, scan, stream)  \

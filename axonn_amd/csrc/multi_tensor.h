@@ -324,13 +324,15 @@ struct Group {
   int blocks;
 };
 
-// Walks the tensor list in launch groups (at most MT_MAX tensors, below 2^31 chunks)
-// and hands each filled argument table to `emit`, which returns a status; the first
-// non-zero status ends the walk.  `ptr_sets[k][i]` is pointer k of tensor i (k = 0 is
-// always the gradient).  Nothing is allocated: the one table lives on the stack.
+// Walks the tensor list in launch groups and hands each filled argument table to `emit`, which
+// returns a status; the first non-zero status ends the walk.  A group has at most MT_MAX tensors
+// and below 2^32 threads, `threads` to a chunk: a launch of more wraps without an error.
+// `ptr_sets[k][i]` is pointer k of tensor i (k = 0 is always the gradient).  Nothing is
+// allocated: the one table lives on the stack.
 template <class Emit>
 int for_each_group(const void* const* const* ptr_sets, const int* elem_sizes, int nsets,
-                   const int64_t* h_sizes, int64_t n, int chunk, Emit&& emit) {
+                   const int64_t* h_sizes, int64_t n, int chunk, int threads, Emit&& emit) {
+  const int64_t most = 0xffffffffLL / threads;
   Group cur;
   cur.tab = MtTable();
   cur.blocks = 0;
@@ -360,12 +362,12 @@ int for_each_group(const void* const* const* ptr_sets, const int* elem_sizes, in
     const int64_t body = sz - head;
     int64_t chunks = (body + chunk - 1) / chunk;
     if (chunks == 0) chunks = 1;  // the head still needs a workgroup
-    if (chunks > 0x3fffffff) {
+    if (chunks > most) {
       set_error("multi-tensor: tensor %lld has too many elements (%lld)",
                 (long long)i, (long long)sz);
       return AXN_ELIMIT;
     }
-    if (k == MT_MAX || (long long)cur.blocks + chunks > 0x7fffffffLL) {
+    if (k == MT_MAX || cur.blocks + chunks > most) {
       const int rc = flush();
       if (rc != AXN_OK) return rc;
     }

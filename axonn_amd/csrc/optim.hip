@@ -456,7 +456,7 @@ int launch_mt_scan(const void* const* h_g, const int64_t* h_sizes, int64_t n,
   const int es[1] = {dtype_size(g_dtype)};
   // first walk: what the partial results need
   int64_t need = 0;
-  int rc = for_each_group(sets, es, 1, h_sizes, n, SCAN_CHUNK, [&](const Group& gr) {
+  int rc = for_each_group(sets, es, 1, h_sizes, n, SCAN_CHUNK, MT_THREADS, [&](const Group& gr) {
     need += gr.blocks;
     return (int)AXN_OK;
   });
@@ -480,7 +480,7 @@ int launch_mt_scan(const void* const* h_g, const int64_t* h_sizes, int64_t n,
   }
   int base = 0;
   bool first = !accumulate;
-  return for_each_group(sets, es, 1, h_sizes, n, SCAN_CHUNK, [&](const Group& gr) {
+  return for_each_group(sets, es, 1, h_sizes, n, SCAN_CHUNK, MT_THREADS, [&](const Group& gr) {
     switch (g_dtype) {
       case AXN_BF16: scan_dispatch<AXN_BF16>(gr, inv_scale, norm_type, partial, base, stream); break;
       case AXN_F16: scan_dispatch<AXN_F16>(gr, inv_scale, norm_type, partial, base, stream); break;
@@ -503,7 +503,7 @@ int launch_mt_scan_noalloc(const void* const* h_g, const int64_t* h_sizes, int64
   const void* const* sets[1] = {h_g};
   const int es[1] = {dtype_size(g_dtype)};
   int64_t need = 0;
-  int rc = for_each_group(sets, es, 1, h_sizes, n, SCAN_CHUNK, [&](const Group& gr) {
+  int rc = for_each_group(sets, es, 1, h_sizes, n, SCAN_CHUNK, MT_THREADS, [&](const Group& gr) {
     need += gr.blocks;
     return (int)AXN_OK;
   });
@@ -560,7 +560,7 @@ int launch_mt_adam(const void* const* h_g, void* const* h_p, void* const* h_m,
   s.hp = hp;
   s.inv_scale = inv_scale;
   const bool has_plow = h_plow != nullptr;
-  return for_each_group(sets, es, 5, h_sizes, n, ADAM_CHUNK, [&](const Group& gr) {
+  return for_each_group(sets, es, 5, h_sizes, n, ADAM_CHUNK, ADAM_THREADS, [&](const Group& gr) {
     switch (g_dtype) {
       case AXN_BF16: return adam_dispatch<AXN_BF16>(gr, s, plow_dtype, has_plow, scan, stream);
       case AXN_F16: return adam_dispatch<AXN_F16>(gr, s, plow_dtype, has_plow, scan, stream);
@@ -574,7 +574,7 @@ int launch_mt_scale(void* const* h_g, const int64_t* h_sizes, int64_t n,
                     int use_clip, hipStream_t stream) {
   const void* const* sets[1] = {(const void* const*)h_g};
   const int es[1] = {dtype_size(g_dtype)};
-  return for_each_group(sets, es, 1, h_sizes, n, SCALE_CHUNK, [&](const Group& gr) {
+  return for_each_group(sets, es, 1, h_sizes, n, SCALE_CHUNK, MT_THREADS, [&](const Group& gr) {
     const dim3 grid(gr.blocks), block(MT_THREADS);
     switch (g_dtype) {
       case AXN_BF16:

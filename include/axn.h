@@ -454,7 +454,8 @@ typedef struct axn_adam_hparams {
  * scan->found_inf != 0 NOTHING is written (the whole step is skipped on the
  * device, axonn/inter_layer.py:428-430), and scan->clip_coef is applied.
  *   h_g/h_p/h_m/h_v/h_plow[n]: device pointers; h_plow may be NULL (no
- *   low-precision copy) ; p, m, v are fp32. */
+ *   low-precision copy) ; p, m, v are fp32.  At most 2^34 - 256 elements to a
+ *   tensor (AXN_ELIMIT). */
 AXN_API int axn_mt_adam(const void* const* h_g, void* const* h_p, void* const* h_m,
                 void* const* h_v, void* const* h_plow, const int64_t* h_sizes,
                 int64_t n, int g_dtype, int plow_dtype, float inv_scale,

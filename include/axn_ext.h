@@ -64,8 +64,8 @@ AXN_API int axn_layer_norm_bwd(const void* dy, const void* h, const void* weight
  *   m += (g - m) * (1 - beta1);  v = v * beta2 + (1 - beta2) * g * g
  *   p = p * keep - lr_over_bc1 * m / (sqrt(v) * inv_sqrt_bc2 + eps)
  *   p_lowp = round_to_nearest_even(p)
- * List, gradient types, scan result and skipped steps as there.  A list whose
- * written tensors overlap is refused (AXN_EINVAL).
+ * List, gradient types, scan result, skipped steps and limit of a tensor as there.
+ * A list whose written tensors overlap is refused (AXN_EINVAL).
  * ------------------------------------------------------------------------ */
 typedef struct axn_adamw_hparams {
   float lr_over_bc1;      /* lr / (1 - beta1^t)          */
