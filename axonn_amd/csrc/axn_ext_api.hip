@@ -39,33 +39,73 @@ int check_param(const char* name, const char* what, const void* p, int bytes) {
     if (rc__) return rc__;   \
   } while (0)
 
-// Two tensors of a list that share elements would be written by two workgroups at once.
-// Tensors in ascending order, as the views of a flat buffer are, are done in one walk.
-// `bytes` for every `unit` elements begun.
-int check_apart(const char* name, const char* what, void* const* h_ptrs, const int64_t* h_sizes, int64_t n, int64_t bytes,
-                int64_t unit = 1) {
-  auto span = [&](int64_t size) { return (uintptr_t)(ceil_div(size, unit) * bytes); };
-  uintptr_t end = 0;
-  int64_t i = 0;
-  for (; i < n; ++i) {
-    if (h_sizes[i] == 0) continue;
-    if ((uintptr_t)h_ptrs[i] < end) break;
-    end = (uintptr_t)h_ptrs[i] + span(h_sizes[i]);
+// One list of a step's tensors: `bytes` for an element, or for every block of them begun.
+struct List {
+  const char* what;
+  const void* const* at;
+  int64_t bytes;
+  bool blocks;
+  uintptr_t begin, end;   // all of the list lies in between
+  uintptr_t from(int64_t i) const { return (uintptr_t)at[i]; }
+  uintptr_t to(int64_t i, const int64_t* h_sizes) const {
+    return from(i) + (uintptr_t)((blocks ? ceil_div(h_sizes[i], AXN_ADAMW8_BLOCK) : h_sizes[i]) * bytes);
   }
-  if (i == n) return AXN_OK;
-  struct Span {
-    uintptr_t begin, end;
-  };
-  Span* spans = new (std::nothrow) Span[n];
+};
+struct Span {
+  uintptr_t begin, end;
+  int list;
+  int64_t tensor;
+};
+
+// Two written tensors that share bytes would be written by two workgroups at once, a gradient that shares
+// some with them would be read by one after another has written it.  A gradient may lie where its own weight
+// or copy does, element for element: a lane reads it before it writes there.
+// Lists in ascending order that lie apart as a whole, as the views of flat buffers do, are done in one walk
+// each.  Lists: gradients, weights, two of the moments, copies.  Two tensors of one list are named first.
+int check_apart(const char* name, List* lists, int count, const int64_t* h_sizes, int64_t n) {
+  bool ascending = true, apart = true;
+  for (int l = 0; l < count; ++l) {
+    List& a = lists[l];
+    uintptr_t last = 0;
+    a.begin = ~(uintptr_t)0, a.end = 0;
+    for (int64_t i = 0; i < n; ++i) {
+      if (h_sizes[i] == 0) continue;
+      const uintptr_t begin = a.from(i), end = a.to(i, h_sizes);
+      ascending = ascending && (l == 0 || begin >= last);   // (gradients are read: two may be the same)
+      last = end;
+      a.begin = std::min(a.begin, begin), a.end = std::max(a.end, end);
+    }
+    for (int k = 0; k < l; ++k) apart = apart && (a.end <= lists[k].begin || lists[k].end <= a.begin);
+  }
+  if (ascending && apart) return AXN_OK;
+  Span* spans = new (std::nothrow) Span[(size_t)n * (count - 1)];
   REQUIRE(spans != nullptr, AXN_ELIMIT, "%s: no host memory to order %lld tensors", name, (long long)n);
   int64_t used = 0;
-  for (i = 0; i < n; ++i)
-    if (h_sizes[i] != 0) spans[used++] = {(uintptr_t)h_ptrs[i], (uintptr_t)h_ptrs[i] + span(h_sizes[i])};
+  for (int l = 1; l < count; ++l)
+    for (int64_t i = 0; i < n; ++i)
+      if (h_sizes[i] != 0) spans[used++] = {lists[l].from(i), lists[l].to(i, h_sizes), l, i};
   std::sort(spans, spans + used, [](const Span& a, const Span& b) { return a.begin < b.begin; });
-  bool apart = true;
-  for (i = 1; i < used && apart; ++i) apart = spans[i - 1].end <= spans[i].begin;
+  // a pair that overlaps: of the written ones two that follow one another (of one list, if there are such)
+  int one = 0, other = 0;
+  for (int64_t i = 1; i < used; ++i)
+    if (spans[i - 1].end > spans[i].begin && (one == 0 || spans[i - 1].list == spans[i].list)) {
+      one = spans[i - 1].list, other = spans[i].list;
+      if (one == other) break;
+    }
+  bool gradient = false;
+  for (int64_t i = 0; i < n && one == 0; ++i) {
+    if (h_sizes[i] == 0) continue;
+    const uintptr_t begin = lists[0].from(i), end = lists[0].to(i, h_sizes);
+    // (written ones are apart by now, so that their ends ascend too)
+    const Span* s = std::upper_bound(spans, spans + used, begin, [](uintptr_t at, const Span& a) { return at < a.end; });
+    if (s == spans + used || s->begin >= end) continue;
+    const bool own = (s->list == 1 || s->list == 4) && s->begin == begin && s->end == end && s->tensor == i;
+    if (!own) one = s->list, gradient = true;
+  }
   delete[] spans;
-  REQUIRE(apart, AXN_EINVAL, "%s: two tensors of %s overlap", name, what);
+  REQUIRE(!gradient, AXN_EINVAL, "%s: a tensor of g and one of %s overlap", name, lists[one].what);
+  REQUIRE(one == 0 || one != other, AXN_EINVAL, "%s: two tensors of %s overlap", name, lists[one].what);
+  REQUIRE(one == 0, AXN_EINVAL, "%s: a tensor of %s and one of %s overlap", name, lists[one].what, lists[other].what);
   return AXN_OK;
 }
 
@@ -144,11 +184,7 @@ static int check_adamw(const char* name, const void* const* h_g, void* const* h_
   REQUIRE(n == 0 || (h_g && h_p && h_m && h_v), AXN_EINVAL, "%s: null pointer array", name);
   CHECK(check_list(name, h_g, "g", h_sizes, n, elem_bytes(g_dtype)));
   CHECK(check_list(name, (const void* const*)h_p, "p", h_sizes, n, 4));
-  CHECK(check_apart(name, "p", h_p, h_sizes, n, 4));
-  if (h_plow != nullptr) {
-    CHECK(check_list(name, (const void* const*)h_plow, "p_lowp", h_sizes, n, 2));
-    CHECK(check_apart(name, "p_lowp", h_plow, h_sizes, n, 2));
-  }
+  if (h_plow != nullptr) CHECK(check_list(name, (const void* const*)h_plow, "p_lowp", h_sizes, n, 2));
   return AXN_OK;
 }
 
@@ -159,8 +195,12 @@ int axn_mt_adamw(const void* const* h_g, void* const* h_p, void* const* h_m, voi
   CHECK(check_adamw(name, h_g, h_p, h_m, h_v, h_plow, h_sizes, n, g_dtype, plow_dtype, hp));
   CHECK(check_list(name, (const void* const*)h_m, "m", h_sizes, n, 4));
   CHECK(check_list(name, (const void* const*)h_v, "v", h_sizes, n, 4));
-  CHECK(check_apart(name, "m", h_m, h_sizes, n, 4));
-  CHECK(check_apart(name, "v", h_v, h_sizes, n, 4));
+  List lists[] = {{"g", h_g, elem_bytes(g_dtype), false},
+                  {"p", (const void* const*)h_p, 4, false},
+                  {"m", (const void* const*)h_m, 4, false},
+                  {"v", (const void* const*)h_v, 4, false},
+                  {"p_lowp", (const void* const*)h_plow, 2, false}};
+  CHECK(check_apart(name, lists, h_plow ? 5 : 4, h_sizes, n));
   return launch_mt_adamw(h_g, h_p, h_m, h_v, h_plow, h_sizes, n, g_dtype, h_plow ? plow_dtype : AXN_BF16, inv_scale, scan,
                          *hp, (hipStream_t)stream);
 }
@@ -175,8 +215,12 @@ int axn_mt_adamw8(const void* const* h_g, void* const* h_p, void* const* h_codes
   for (int64_t i = 0; i < n; ++i)
     REQUIRE(ceil_div(h_sizes[i], AXN_ADAMW8_BLOCK) < (1 << 26), AXN_ELIMIT, "%s: tensor %lld has too many elements (%lld)",
             name, (long long)i, (long long)h_sizes[i]);
-  CHECK(check_apart(name, "codes", h_codes, h_sizes, n, 2 * AXN_ADAMW8_BLOCK, AXN_ADAMW8_BLOCK));
-  CHECK(check_apart(name, "exponents", h_exponents, h_sizes, n, 2, AXN_ADAMW8_BLOCK));
+  List lists[] = {{"g", h_g, elem_bytes(g_dtype), false},
+                  {"p", (const void* const*)h_p, 4, false},
+                  {"codes", (const void* const*)h_codes, 2 * AXN_ADAMW8_BLOCK, true},
+                  {"exponents", (const void* const*)h_exponents, 2, true},
+                  {"p_lowp", (const void* const*)h_plow, 2, false}};
+  CHECK(check_apart(name, lists, h_plow ? 5 : 4, h_sizes, n));
   return launch_mt_adamw8(h_g, h_p, h_codes, h_exponents, h_plow, h_sizes, n, g_dtype, h_plow ? plow_dtype : AXN_BF16,
                           inv_scale, seed, scan, *hp, (hipStream_t)stream);
 }

@@ -65,7 +65,9 @@ AXN_API int axn_layer_norm_bwd(const void* dy, const void* h, const void* weight
  *   p = p * keep - lr_over_bc1 * m / (sqrt(v) * inv_sqrt_bc2 + eps)
  *   p_lowp = round_to_nearest_even(p)
  * List, gradient types, scan result, skipped steps and limit of a tensor as there.
- * A list whose written tensors overlap is refused (AXN_EINVAL).
+ * Refused (AXN_EINVAL): written tensors that overlap, of one list or of two, and a
+ * gradient that overlaps one, unless it lies where its own weight or copy does,
+ * element for element.
  * ------------------------------------------------------------------------ */
 typedef struct axn_adamw_hparams {
   float lr_over_bc1;      /* lr / (1 - beta1^t)          */

@@ -37,3 +37,29 @@ def test_lazy_clones_of_what_a_step_writes_stay(bits, as_list):
         for a, b in zip(step(*lazy), want):
             assert torch.equal(a, b), which
         assert torch.equal(twins[which], start[which]), which
+
+
+def test_lists_that_share_memory_are_refused():
+    """And nothing of them is written."""
+    from axonn_amd import ops
+
+    hp = ops.adamw_hparams(1, 1e-2, 0.9, 0.999, 1e-8, 0.1)
+    flat = torch.randn(4096, device="cuda")
+    g, p, m, v = flat[:1000], flat[1000:2000], flat[2000:3000], flat[3000:4000]
+    spare = torch.zeros(4096, device="cuda", dtype=torch.uint8)
+    codes, exponents = spare[:2048], torch.zeros(8, device="cuda", dtype=torch.uint8)
+    before = flat.clone()
+    for lists in (([g], [p], [m], [m]), ([g], [p], [p], [v]), ([g], [p], [m], [flat[2999:3999]]),
+                  ([flat[1:1001]], [g], [m], [v]), ([m], [p], [m], [v])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.mt_adamw(*lists, None, hp)
+    for lists in (([p], [p], [codes], [codes[:8]]), ([g], [spare[96:].view(torch.float32)], [codes], [exponents])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.mt_adamw8(*lists, None, hp, 0)
+    assert torch.equal(flat, before) and not spare.any()
+    # the copy in the gradients' place, as apart from them
+    low, apart = g.bfloat16(), torch.empty(1000, device="cuda", dtype=torch.bfloat16)
+    args = [(low.clone(), p.clone(), m.clone(), v.abs()) for _ in range(2)]
+    ops.mt_adamw(*([t] for t in args[0]), [apart], hp)
+    ops.mt_adamw(*([t] for t in args[1]), [args[1][0]], hp)
+    assert torch.equal(args[1][0], apart) and all(torch.equal(a, b) for a, b in zip(args[0][1:], args[1][1:]))
