@@ -43,7 +43,7 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, residual=N
     """F.layer_norm with the same arguments, on the HIP kernels.  With `residual`: (norm(x + residual), x + residual),
     the sum rounded to its type and normalised as it is rounded.
 
-    Parameters are of x's type or fp32; under autocast the norm is fp32, as torch's is."""
+    Parameters are of x's type or fp32; under autocast the norm is fp32, as torch's is (64 bits are refused with and without)."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     if not shape or tuple(x.shape[x.dim() - len(shape):]) != shape:
         raise ValueError("layer_norm: expected the last dimensions to be %s, got %s" % (shape, tuple(x.shape)))
@@ -53,7 +53,8 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, residual=N
     if residual is not None and residual.shape != x.shape:
         raise ValueError("layer_norm: residual is %s, expected %s" % (tuple(residual.shape), tuple(x.shape)))
     if torch.is_autocast_enabled("cuda"):
-        x, residual, weight, bias = (t if t is None else t.float() for t in (x, residual, weight, bias))
+        x, residual, weight, bias = (t.float() if t is not None and t.dtype in (torch.float16, torch.bfloat16) else t
+                                     for t in (x, residual, weight, bias))
     rows, n = x.shape, math.prod(shape)
     as_rows = [t if t is None else t.reshape(-1, n) for t in (x, residual)]
     params = [p if p is None else p.reshape(-1) for p in (weight, bias)]

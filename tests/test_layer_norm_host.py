@@ -70,3 +70,21 @@ def test_a_trace_computes_what_the_layer_does(launches, gradients, with_residual
             got, want = traced(*args), layer(*args)
         for a, b in zip(*((got, want) if with_residual else ((got,), (want,)))):
             assert torch.equal(a, b) and a.requires_grad == again
+
+
+@pytest.mark.parametrize("which", ["x", "residual", "weight", "bias"])
+def test_autocast_leaves_64_bits_as_they_are(launches, monkeypatch, which):
+    """Autocast widens 16 bits to 32; 64 bits, which the kernels do not have, reach their check of types and are not
+    made 32 on the way."""
+    seen = []
+    forward = ops.layer_norm_fwd
+    monkeypatch.setattr(ops, "layer_norm_fwd", lambda x, weight, bias, eps, residual=None, save=True: (
+        seen.append([t.dtype for t in (x, residual, weight, bias)]), forward(x, weight, bias, eps, residual, save))[1])
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda *device: True)
+    args = dict(x=torch.randn(3, 8).half(), residual=torch.randn(3, 8).bfloat16(), weight=torch.ones(8), bias=torch.zeros(8).half())
+    for gradients in (True, False):
+        with torch.set_grad_enabled(gradients):
+            layer_norm(normalized_shape=8, **args)
+            assert seen.pop() == [torch.float32] * 4
+            layer_norm(normalized_shape=8, **{**args, which: args[which].double()})
+            assert seen.pop() == [torch.float64 if w == which else torch.float32 for w in args]
