@@ -263,7 +263,10 @@ class AdamW(CPUAdam):
     8 bits with an exponent byte for each 256 elements and moment (`codes`, `exponents`; 2 bytes an
     element instead of 8).  Codes are rounded stochastically, `seed` and the step's number make the
     random words: runs with equal seeds are equal bit by bit.  Every parameter then starts at a
-    whole block, so `model_params_fp32` and its like have zeros between the parameters."""
+    whole block, so `model_params_fp32` and its like have zeros between the parameters.
+
+    `state_dict()` holds all that the next step depends on, so that a run goes on bit by bit where it
+    was saved; its tensors are the optimizer's own, as torch's are."""
 
     def __init__(
         self,
@@ -310,6 +313,49 @@ class AdamW(CPUAdam):
         else:
             m, v = self._parts(lo, hi, self.exp_avg, self.exp_avg_sq)
             ops.mt_adamw(g, p, m, v, low, hp, inv_scale=inv_scale, scan=scan)
+
+    # -- saved states -------------------------------------------------------
+    def _saved_tensors(self):
+        return ["model_params_fp32"] + (["exp_avg", "exp_avg_sq"] if self.state_bits == 32 else ["codes", "exponents"])
+
+    def state_dict(self):
+        """torch's, whose param groups have no state of their own, and "flat": the fp32 weights, the
+        moments or their codes, the step's number, the seed and the loss scale."""
+        state = super().state_dict()
+        state["flat"] = {
+            "state_bits": self.state_bits,
+            "sizes": [[p.numel() for p in group["params"]] for group in self.param_groups],
+            "step_count": self.step_count,
+            "seed": self.seed,
+            "scaler": {field: getattr(self.scaler, field) for field in LossScaler.__dataclass_fields__},
+            **{name: getattr(self, name) for name in self._saved_tensors()},
+        }
+        return state
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """Takes the state in place: the weights of the model are then those of the saved fp32 weights.
+        One of other sizes or another `state_bits`, or without moments, is refused as a whole."""
+        flat = state_dict.get("flat")
+        if flat is None:
+            raise ValueError("AdamW: the saved state holds neither moments nor weights")
+        if flat["state_bits"] != self.state_bits:
+            raise ValueError("AdamW: the saved moments have %s bits, this optimizer's %d" % (flat["state_bits"], self.state_bits))
+        if flat["sizes"] != [[p.numel() for p in group["params"]] for group in self.param_groups]:
+            raise ValueError("AdamW: the saved state is that of parameters of other sizes, or in other groups")
+        for name in self._saved_tensors():
+            saved, mine = flat[name], getattr(self, name)
+            if saved.shape != mine.shape or saved.dtype != mine.dtype:
+                raise ValueError("AdamW: saved %s is %s %s, expected %s %s" % (name, saved.dtype, tuple(saved.shape), mine.dtype,
+                                                                              tuple(mine.shape)))
+        super().load_state_dict({name: value for name, value in state_dict.items() if name != "flat"})
+        for name in self._saved_tensors():
+            getattr(self, name).copy_(flat[name])
+        if self._writes_lowp:
+            self.model_params_fp16.copy_(self.model_params_fp32)   # (rounded as the step does)
+        self.step_count, self.seed = flat["step_count"], flat["seed"]
+        for field, value in flat["scaler"].items():
+            setattr(self.scaler, field, value)
 
     def moments(self):
         """(exp_avg, exp_avg_sq) of every parameter, in fp32 and its shape: with 32 bits views of the
