@@ -283,13 +283,20 @@ class AdamW(CPUAdam):
     ):
         if state_bits not in (8, 32):
             raise ValueError("Invalid number of bits of the moments: {}".format(state_bits))
-        if state_bits == 8 and not eps > 0.0:
-            raise ValueError("8-bit moments need a positive epsilon, got {}".format(eps))
         self.state_bits, self.seed = state_bits, int(seed)
         if state_bits == 8:
             self._span = lambda n: -(-n // nv.ADAMW8_BLOCK) * nv.ADAMW8_BLOCK
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm,
                          loss_scaler=loss_scaler, dynamic_loss_scale=dynamic_loss_scale)
+
+    def _check_eps(self, eps):
+        if self.state_bits == 8 and not eps > 0.0:
+            raise ValueError("8-bit moments need a positive epsilon, got {}".format(eps))
+
+    def add_param_group(self, param_group):   # (torch's constructor adds every group by it)
+        if isinstance(param_group, dict):     # (anything else torch refuses)
+            self._check_eps(param_group.get("eps", self.defaults["eps"]))
+        super().add_param_group(param_group)
 
     def _make_moments(self, total, device):
         if self.state_bits == 8:
@@ -348,6 +355,8 @@ class AdamW(CPUAdam):
             if saved.shape != mine.shape or saved.dtype != mine.dtype:
                 raise ValueError("AdamW: saved %s is %s %s, expected %s %s" % (name, saved.dtype, tuple(saved.shape), mine.dtype,
                                                                               tuple(mine.shape)))
+        for group in state_dict["param_groups"]:
+            self._check_eps(group["eps"])
         super().load_state_dict({name: value for name, value in state_dict.items() if name != "flat"})
         for name in self._saved_tensors():
             getattr(self, name).copy_(flat[name])

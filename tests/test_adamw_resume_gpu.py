@@ -90,3 +90,12 @@ def test_states_that_do_not_fit_are_refused(bits):
             opt.load_state_dict(bad)
     assert opt.step_count == 1 and opt.param_groups[0]["lr"] == 1e-2 * 0.9
     assert all(torch.equal(a, b) for a, b in zip(before, everything(params, opt)))
+
+
+def test_a_saved_group_without_eps_is_refused_by_8_bit_moments():
+    params, opt = fresh(torch.bfloat16, 8, 0)
+    state = opt.state_dict()
+    state["param_groups"][1]["eps"] = 0.0
+    with pytest.raises(ValueError, match="positive"):
+        opt.load_state_dict(state)
+    assert opt.param_groups[1]["eps"] == 1e-8
