@@ -79,12 +79,6 @@ __device__ __forceinline__ int exponent_of(uint32_t bits) {
   const uint32_t e = (bits + 0x100000u) >> 23;
   return e > NOT_FINITE ? NOT_FINITE : (int)e;
 }
-// The code of a magnitude of at most E's, `word`'s 16 bits being the place from which on the
-// upper one of its two neighbours is taken.
-__device__ __forceinline__ uint32_t encode(float magnitude, int e, int bias, uint32_t word) {
-  return (__float_as_uint(ldexpf(magnitude, bias - e)) + (word << 4 | 8u)) >> 20;
-}
-
 // The random words of the four elements q * 4 ... of the list: a counter, two keys, two
 // rounds of multiplying and folding (odd constants from the golden ratio and the square roots
 // of 2, 3, 11, 17 and 19).  The low half is the first moment's, the high one the second's.
@@ -189,7 +183,8 @@ __device__ __forceinline__ u32x2 encode4(const Four& x, int em, int ev, const ui
   uint32_t m[4], v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    // a code's bits are 20 to 27 of the sum; 4 up they are the top byte, the sign above the code
+    // (a magnitude of at most E's; the word's 16 bits are the place from which on the upper one of its two neighbours is
+    // taken) a code's bits are 20 to 27 of the sum; 4 up they are the top byte, the sign above the code
     m[e] = (__float_as_uint(ldexpf(fabsf(x.m[e]), M_BIAS - em)) + (words[e] << 4 & 0xffff0u | 8u)) << 4;
     m[e] |= x.m[e] < 0.0f ? 0x80000000u : 0u;
     v[e] = (__float_as_uint(ldexpf(x.v[e], V_BIAS - ev)) + (words[e] >> 12 & 0xffff0u | 8u)) << 4;
