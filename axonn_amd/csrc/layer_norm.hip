@@ -31,8 +31,8 @@ __device__ __forceinline__ float param_at(const void* p, int wide, int64_t i) {
 
 constexpr int64_t kL2 = 32 << 20;        // bytes that the eight L2s hold
 // Bytes that the memory-side cache holds.  A forward with a residual that moves more keeps nothing in the
-// caches, in two turns a workgroup: 16384 x 8192 bf16 203 -> 180 us, with the product that reads it 368 ->
-// 374 (8192 x 8192 215 -> 206, 32768 x 8192 753 -> 739).  Without a residual there is nothing in it (98 us
+// caches, in two turns a workgroup: 16384 x 8192 bf16 203 -> 181 us on the same rows again and again (187 on
+// others every time), with the product that reads it 368 -> 374 (8192 x 8192 215 -> 206, 32768 x 8192 753 -> 739).  Without a residual there is nothing in it (98 us
 // -> 105, 279 -> 299).
 constexpr int64_t kCached = 256 << 20;
 constexpr int MOST_PARTS = 256;   // parts of the rows whose column sums meet in a second launch
@@ -60,7 +60,9 @@ struct NormGradArgs {
 // same GPU moves 6.8 TB/s; the forward moves 5.1 to 5.9 TB/s of bf16 from 20 MB on, the backward 4 to
 // 5.5 (see there).
 // A row lies in the registers of 16 lanes or of several whole waves, K vectors of 16 bytes in a
-// lane, and is read once.
+// lane, and is read once.  With four of them, rows of 16385 to 32768 16-bit elements, 128 registers do not
+// hold it all: the forward with a residual spills 36 to 84 bytes a lane, the backward 148 to 224 (fp32,
+// 8193 to 16384 elements: 16 to 24 with dsum; two vectors of 16 lanes with dsum: 12 to 20).
 // Vector v of a row holds its elements from v VEC on, but the last one ends with the row and
 // overlaps the one before: `twice` of its elements are in both, count once in sums and are
 // stored by both with one value.  Rows may start anywhere: the accesses are declared to be
@@ -357,6 +359,10 @@ int norm_rows(const NormArgs& a, hipStream_t stream) {
 // that adds them up.  256 workgroups of up to 16 waves, one to a CU, are a compromise: 512 of half the
 // size, two to a CU, are 5 % faster up to their sums and 5 to 15 % slower with twice as many of those.
 // 4096 x 4096 bf16 with dsum 32.7 us (4.1 TB/s), 16384 x 5120 98 us (5.1), 32768 x 4096 147 us (5.5).
+// Wider rows fill a CU with one workgroup and its partial sums grow: 16384 x 8192 bf16 149 us (5.4), 8192 x
+// 16384 160 us (5.0), 16384 x 8192 fp32 295 us (5.5).  Four vectors to a lane, which spill, fall off:
+// 4096 x 24576 bf16 222 us (2.7), 4096 x 32768 286 us (2.8), 600 x 32768 86 us, where the kernels of long
+// rows take 335 and 54 us for eight elements more; 4096 x 16384 fp32 162 us (5.0), and 313 for four more.
 // Rows as above, several at a time in a workgroup, which goes on to the rows `parts`
 // workgroups further until there are none.  Its threads keep the sums of dy xhat and dy of their
 // columns in registers; at the end the workgroup's rows are joined in LDS and its sums go to
@@ -738,7 +744,10 @@ __global__ void __launch_bounds__(FEW_THREADS) norm_grad_few_kernel(const NormGr
 // Up to 512 rows (of 16 elements on, so that a vector fits, and up to 2^20, so that the grid does).  us, two
 // launches / this one: 64 x 1024 fp32 7.4 / 5.0, 400 x 1024 10.1 / 6.0, 800 x 1024 10.6 / 11.3; 256 x 4096 bf16 10.6 / 5.5, 800 x 4096
 // 14.7 / 12.5, 1100 x 4096 16.4 / 15.8; 128 x 12288 16.4 / 10.2, 600 x 12288 21.4 / 19.7, 800 x 12288 23.9 /
-// 27.0; 400 x 8192 fp32 14.7 / 13.8, 600 x 8192 17.1 / 20.3.
+// 27.0; 400 x 8192 fp32 14.7 / 13.8, 600 x 8192 17.1 / 20.3.  At the rule's border, 513 rows in two launches
+// / 512 in this one: bf16 x 1024 10.2 / 5.7, x 8192 16.7 / 10.5, x 16384 24.0 / 23.1, x 65536 89 / 88, x 2^20
+// 1823 / 1699; fp32 x 1024 9.7 / 6.0, x 8192 16.5 / 16.9, x 16384 27.6 / 33.3, x 65536 174 / 137, x 2^20 3555
+// / 2855.  So the rule loses on fp32 rows of some 8192 to 16384 elements, from 450 and 400 rows on.
 inline bool few_rows(int64_t M, int64_t N) { return M >= 1 && M <= 512 && N >= 16 && N <= 1 << 20; }
 
 template <typename T>

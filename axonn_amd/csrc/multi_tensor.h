@@ -28,7 +28,7 @@ constexpr int ADAM_THREADS = 64;                // lanes per workgroup of the up
 constexpr int ADAM_VECS = 1;                    // vectors per lane
 constexpr int ADAM_CHUNK = ADAM_THREADS * ADAM_VEC * ADAM_VECS;
 // LDS the update kernel reserves per workgroup and never touches: it bounds the
-// workgroups that are resident on a CU (160 KB per CU), see mt_adam_kernel.
+// workgroups that are resident on a CU (160 KB per CU), see update_chunk.
 constexpr int ADAM_LDS = 15360;
 // Cache policy bits of the update kernel's buffer accesses (1 sc0, 2 nt, 16 sc1).  Loads
 // non-temporal; stores non-temporal and written through (nt + sc1): 1 to 2 % over nt
@@ -54,7 +54,7 @@ struct MtTable {
   int32_t meta[MT_MAX];             // bits 0-7: scalar elements before the aligned body;
                                     // bit 8: vector accesses allowed
   int32_t n;
-  int32_t chunk;                    // elements per workgroup (multiple of MT_VEC)
+  int32_t chunk;                    // elements per workgroup (a multiple of 8)
 };
 
 __device__ __forceinline__ int head_of(const MtTable& t, int i) { return t.meta[i] & 0xff; }

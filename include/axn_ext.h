@@ -95,7 +95,8 @@ AXN_API int axn_mt_adamw(const void* const* h_g, void* const* h_p, void* const* 
  *   m = +-F(c & 127) * 2^(E - 141),  v = F(c) * 2^(E - 157)
  * E is the exponent field of the block's largest magnitude as a float, the next one
  * if its mantissa is 1.875 or more.  Zeroed codes and exponents are zero moments.
- * E = 255: the block is not finite (a gradient was not); all of it reads as NaN.
+ * E = 255: the block is not finite (a gradient was not, or a moment came to 1.875 * 2^127);
+ * all of it reads as NaN.
  * m and v of the step are rounded to codes stochastically: the upper one of the two
  * neighbours is taken from (u + 1/2) / 2^16 <= their distance to the lower one on, u
  * 16 bits of a word that seed (64 bits) and the element's place give; a v above zero
